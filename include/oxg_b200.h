@@ -101,6 +101,74 @@ OXG_API int oxg_dequant_mxfp4(oxg_ctx *ctx, const uint8_t *blocks_dev, size_t n_
 OXG_API int oxg_swiglu(oxg_ctx *ctx, const float *gate_dev, const float *up_dev, size_t n,
                        float alpha, float limit, float *out_dev);
 
+/* ---- MXFP4 operands: quantisation and products ---------------------------
+ * No counterpart in the reference, which dequantises its weights
+ * (src/mxfp4.rs:15-54) and multiplies in f16. An MXFP4 operand is a matrix
+ * of rows of k elements (k a multiple of 32): packed codes [rows, k/2] as
+ * oxg_dequant_mxfp4 takes them and one E8M0 scale byte for each 32 elements,
+ * in one of two layouts:
+ *   OXG_SCALES_ROWS   [rows, k/32], the checkpoint's order;
+ *   OXG_SCALES_TILED  [ceil(k/128)][rows][4], what the products read: the
+ *                     four bytes of a row's 128-element stretch, consecutive
+ *                     rows side by side (4-byte aligned; where k ends inside a
+ *                     stretch the bytes past it must not be 255, and are
+ *                     written as 0 here). A weight is laid out once with
+ *                     oxg_mxfp4_tile_scales; the quantisers write either.
+ * These calls keep nothing between them and use no workspace: calls on several
+ * streams, or replays of several captured graphs, do not disturb one another. */
+enum { OXG_DTYPE_F32 = 0, OXG_DTYPE_BF16 = 1, OXG_DTYPE_F16 = 2 };
+/* A block with largest magnitude t in [2^e, 2^(e+1)) gets the scale 2^(e-2)
+ * (FLOOR: what then lies above E2M1's largest value 6 becomes 6), or twice
+ * that where t > 1.5 * 2^e (NOCLIP: nothing lies above 6); never below 2^-126,
+ * and never above 2^125 (6 * 2^126 would not be finite in f32). */
+enum { OXG_MX_FLOOR = 0, OXG_MX_NOCLIP = 1 };
+enum { OXG_SCALES_ROWS = 0, OXG_SCALES_TILED = 1 };
+
+/* The inverse of oxg_dequant_mxfp4: x_dev [rows, cols] of `dtype`, ld elements
+ * from row to row, each row times row_scale_dev[row] (f32, may be NULL; an f32
+ * product) -> blocks_dev [rows, cols/2] (4-byte aligned) and scales_dev.
+ * Each element becomes the nearest E2M1 value times the block's scale, ties to
+ * the even code. A block holding an infinity or a NaN becomes codes 0 with
+ * scale byte 255, which reads as NaN. */
+OXG_API int oxg_quantize_mxfp4(oxg_ctx *ctx, const void *x_dev, int dtype, size_t rows, size_t cols, size_t ld,
+                               const float *row_scale_dev, int scale_rule, int scale_layout, uint8_t *blocks_dev,
+                               uint8_t *scales_dev);
+
+/* oxg_swiglu's function of gate_up_dev [rows, 2*cols] (gate in the even
+ * columns, up in the odd ones, as the expert products lay them out), quantised
+ * as above. The codes are those of the exact value: where f32 arithmetic
+ * could fall on the other side of a border the block is evaluated in f64. */
+OXG_API int oxg_swiglu_quantize_mxfp4(oxg_ctx *ctx, const void *gate_up_dev, int dtype, size_t rows, size_t cols,
+                                      size_t ld, float alpha, float limit, int scale_rule, int scale_layout,
+                                      uint8_t *blocks_dev, uint8_t *scales_dev);
+
+/* scales_dev [n_groups, rows, cols/32] -> tiled_dev [n_groups, ceil(cols/128), rows, 4]. */
+OXG_API int oxg_mxfp4_tile_scales(oxg_ctx *ctx, const uint8_t *scales_dev, size_t n_groups, size_t rows, size_t cols,
+                                  uint8_t *tiled_dev);
+
+/* out[i][j] = sum over k of a[i][k] * b[j][k], plus bias[j] (bf16 [n], may be
+ * NULL), for MXFP4 operands a [m, k] and b [n, k] (blocks 16-byte aligned,
+ * scales OXG_SCALES_TILED): the tensor cores' E2M1 product, f32 sums, rounded
+ * once where out_dtype is OXG_DTYPE_BF16 (else OXG_DTYPE_F32); ldo elements
+ * from one row of out to the next. Scale bytes mean what the MX format says:
+ * 2^(e-127), and NaN for 255 (oxg_dequant_mxfp4 follows the reference, which
+ * has 0 -> 0.0 and 255 -> inf; the quantisers never write 0). */
+OXG_API int oxg_mxfp4_matmul(oxg_ctx *ctx, const uint8_t *a_blocks_dev, const uint8_t *a_scales_dev, int m,
+                             const uint8_t *b_blocks_dev, const uint8_t *b_scales_dev, int n, int k,
+                             const uint16_t *bias_dev, void *out_dev, int out_dtype, size_t ldo);
+
+/* The same with a matrix b for each of n_groups (<= 1024) runs of consecutive
+ * rows of a: counts_dev [n_groups] int32 (device, as oxg_moe_dispatch writes
+ * them; zeros allowed) rows each, b_blocks_dev [n_groups, n, k/2], its scales
+ * [n_groups, ceil(k/128), n, 4], bias_dev [n_groups, n] or NULL. m is the
+ * number of rows a and out have room for; rows past the last group are left as
+ * they were. A negative count (taken as 0) or counts beyond m (cut off there)
+ * make the next oxg_sync return OXG_ERR_SHAPE. */
+OXG_API int oxg_mxfp4_grouped_matmul(oxg_ctx *ctx, const uint8_t *a_blocks_dev, const uint8_t *a_scales_dev, int m,
+                                     const int32_t *counts_dev, int n_groups, const uint8_t *b_blocks_dev,
+                                     const uint8_t *b_scales_dev, int n, int k, const uint16_t *bias_dev,
+                                     void *out_dev, int out_dtype, size_t ldo);
+
 /* ---- MoE layer ----------------------------------------------------------- */
 
 typedef struct {

@@ -31,6 +31,13 @@ OXG_MODE_DECODE = 1
 OXG_MODE_PREFILL = 2
 OXG_MODE_MXF4 = 3
 OXG_PRECISION_PARITY = 0
+OXG_DTYPE_F32 = 0
+OXG_DTYPE_BF16 = 1
+OXG_DTYPE_F16 = 2
+OXG_MX_FLOOR = 0
+OXG_MX_NOCLIP = 1
+OXG_SCALES_ROWS = 0
+OXG_SCALES_TILED = 1
 
 
 class OxgError(RuntimeError):
@@ -81,6 +88,11 @@ SIGNATURES = {
     "oxg_sync": (_I, [_CTX]),
     "oxg_dequant_mxfp4": (_I, [_CTX, _P, _SZ, _P, _SZ, _I, _SZ, _SZ, _P]),
     "oxg_swiglu": (_I, [_CTX, _P, _P, _SZ, ctypes.c_float, ctypes.c_float, _P]),
+    "oxg_quantize_mxfp4": (_I, [_CTX, _P, _I, _SZ, _SZ, _SZ, _P, _I, _I, _P, _P]),
+    "oxg_swiglu_quantize_mxfp4": (_I, [_CTX, _P, _I, _SZ, _SZ, _SZ, ctypes.c_float, ctypes.c_float, _I, _I, _P, _P]),
+    "oxg_mxfp4_tile_scales": (_I, [_CTX, _P, _SZ, _SZ, _SZ, _P]),
+    "oxg_mxfp4_matmul": (_I, [_CTX, _P, _P, _I, _P, _P, _I, _I, _P, _P, _I, _SZ]),
+    "oxg_mxfp4_grouped_matmul": (_I, [_CTX, _P, _P, _I, _P, _I, _P, _P, _I, _I, _P, _P, _I, _SZ]),
     "oxg_moe_upload": (_I, [_CTX, _I, ctypes.POINTER(MoeDims), ctypes.POINTER(MoeWeights)]),
     "oxg_moe_release": (_I, [_CTX, _I]),
     "oxg_moe_reserve": (_I, [_CTX, _I, _I]),

@@ -1,0 +1,55 @@
+// mx4.h — host-side launchers of the MXFP4 operators: quantisation
+// (mx4_quant.cu) and the products of two MXFP4 operands (mx4_gemm.cu).
+// Internal to the library.
+#pragma once
+
+#include <cuda_runtime.h>
+#include <stddef.h>
+#include <stdint.h>
+
+namespace oxg {
+
+// Element types and scale rules and layouts, as the public header numbers them.
+enum { kMx4F32 = 0, kMx4Bf16 = 1, kMx4F16 = 2 };
+enum { kMx4Floor = 0, kMx4NoClip = 1 };
+enum { kMx4ScaleRows = 0, kMx4ScaleTiled = 1 };
+
+struct Mx4QuantArgs {
+  const void *x = nullptr;           // [rows, cols] (SwiGLU: [rows, 2 cols], gate and up interleaved)
+  size_t ld = 0;                     // elements from one row to the next
+  size_t rows = 0, cols = 0;         // of the quantised matrix; cols a multiple of 32
+  const float *row_scale = nullptr;  // [rows] factors, or null
+  int rule = kMx4Floor;
+  int tiled = 0;
+  float alpha = 0.f, limit = 0.f;    // SwiGLU
+  uint8_t *blocks = nullptr;         // [rows, cols / 2], 4-byte aligned
+  uint8_t *scales = nullptr;         // [rows, cols / 32], or tiled [ceil(cols / 128), rows, 4]
+};
+cudaError_t launch_mx4_quantize(const Mx4QuantArgs &a, int dtype, bool swiglu, int n_sms, cudaStream_t stream);
+
+// Scale rows [groups, rows, cols / 32] -> tiled [groups, ceil(cols / 128), rows, 4].
+cudaError_t launch_mx4_tile_scales(const uint8_t *src, size_t groups, size_t rows, size_t cols, uint8_t *dst, int n_sms,
+                                   cudaStream_t stream);
+
+constexpr int kMx4MaxGroups = 1024;
+// Error-word codes of the products.
+constexpr int kMx4ErrWait = 81;    // a pipeline wait ran out
+constexpr int kMx4ErrCounts = 85;  // a negative group count, or counts beyond the rows there are
+
+struct Mx4GemmArgs {
+  int m = 0, n = 0, k = 0;           // activation rows, weight rows (per group), reduction length
+  int groups = 1;
+  const int32_t *counts = nullptr;   // [groups] rows of each group (device), or null: one group of m rows
+  const uint8_t *a = nullptr;        // [m, k / 2] codes
+  const uint32_t *a_scales = nullptr;  // [ceil(k / 128), m]
+  const uint8_t *b = nullptr;        // [groups, n, k / 2] codes
+  const uint32_t *b_scales = nullptr;  // [groups, ceil(k / 128), n]
+  const uint16_t *bias = nullptr;    // [groups, n] bf16, or null
+  void *out = nullptr;               // [m, ldo]
+  size_t ldo = 0;
+  int out_bf16 = 0;                  // else f32
+  int *err = nullptr;
+};
+cudaError_t launch_mx4_gemm(const Mx4GemmArgs &a, int n_sms, cudaStream_t stream);
+
+}  // namespace oxg

@@ -1,0 +1,307 @@
+// mx4_quant.cu — floating-point rows to MXFP4, alone or behind the clamped SwiGLU.
+//
+// A block of 32 elements with largest magnitude t gets the scale
+//   floor rule:   s = 2^(floor(log2 t) - 2)       (t / s in [4, 8): what lies above 6 becomes 6)
+//   noclip rule:  twice that where t > 1.5 * 2^floor(log2 t)   (t / s in (3, 6]: nothing clips)
+// but at least 2^-126, so that the byte 0, which means 0.0 to the dequantisation and 2^-127 to the tensor
+// cores, never comes up, and at most 2^125, so that what was finite reads back finite (4 * 2^126 would not
+// in f32 or bf16). Each element becomes the E2M1 value nearest to x / s, ties to the even code
+// (cvt.rn.satfinite.e2m1x2; x / s is exact, s being a power of two). A block that holds an infinity or a
+// NaN becomes codes 0 under scale byte 255, which reads as NaN everywhere.
+//
+// Bound: HBM. A thread owns 8 consecutive elements (one 16-byte load of 16-bit types, two of f32) and a
+// block is four neighbouring lanes, which share the largest magnitude by two shuffles; the codes leave as
+// one 4-byte word per thread. Each thread issues the loads of kUnr chunks, a grid's width apart, before it
+// works on the first.
+#include "common.cuh"
+#include "mx4.h"
+
+namespace oxg {
+namespace {
+
+constexpr int kThreads = 256;
+
+template <int T>
+struct Elem;
+template <>
+struct Elem<kMx4F32> {
+  static constexpr int kBytes = 4;
+};
+template <>
+struct Elem<kMx4Bf16> {
+  static constexpr int kBytes = 2;
+};
+template <>
+struct Elem<kMx4F16> {
+  static constexpr int kBytes = 2;
+};
+
+// N consecutive elements as raw 16-byte words. Without VEC (a base or a row pitch off the 16-byte grid)
+// they are read one by one.
+template <int T, int N, bool VEC>
+struct Raw {
+  static constexpr int kWords = N * Elem<T>::kBytes / 16;
+  uint4 w[kWords];
+  __device__ __forceinline__ void load(const void *p) {
+    if (VEC) {
+#pragma unroll
+      for (int i = 0; i < kWords; ++i) w[i] = ldg_stream_v4(static_cast<const uint4 *>(p) + i);
+    } else if (Elem<T>::kBytes == 4) {
+      uint32_t *d = reinterpret_cast<uint32_t *>(w);
+#pragma unroll
+      for (int i = 0; i < N; ++i) d[i] = __ldg(static_cast<const uint32_t *>(p) + i);
+    } else {
+      uint32_t *d = reinterpret_cast<uint32_t *>(w);
+      const uint16_t *s = static_cast<const uint16_t *>(p);
+#pragma unroll
+      for (int i = 0; i < N / 2; ++i) d[i] = (uint32_t)__ldg(s + 2 * i) | ((uint32_t)__ldg(s + 2 * i + 1) << 16);
+    }
+  }
+  __device__ __forceinline__ void values(float (&v)[N]) const {
+    const uint32_t *d = reinterpret_cast<const uint32_t *>(w);
+    if (T == kMx4F32) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) v[i] = __uint_as_float(d[i]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < N / 2; ++i) {
+        if (T == kMx4Bf16) {
+          v[2 * i] = __uint_as_float(d[i] << 16);
+          v[2 * i + 1] = __uint_as_float(d[i] & 0xFFFF0000u);
+        } else {
+          const float2 f = unpack_f16x2(d[i]);
+          v[2 * i] = f.x;
+          v[2 * i + 1] = f.y;
+        }
+      }
+    }
+  }
+};
+
+// Eight values to four code bytes, element 0 in the lowest half byte.
+__device__ __forceinline__ uint32_t e2m1_pack8(const float (&v)[8]) {
+  uint32_t r;
+  asm("{\n\t.reg .b8 b0, b1, b2, b3;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 b0, %2, %1;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 b1, %4, %3;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 b2, %6, %5;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 b3, %8, %7;\n\t"
+      "mov.b32 %0, {b0, b1, b2, b3};\n\t}"
+      : "=r"(r)
+      : "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7]));
+  return r;
+}
+__device__ __forceinline__ uint32_t pack_scaled(const float (&v)[8], float f) {
+  float r[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) r[i] = v[i] * f;
+  return e2m1_pack8(r);
+}
+
+// Scale byte of a block from the f32 bits of its largest magnitude (finite).
+__device__ __forceinline__ int scale_byte(uint32_t top, int rule) {
+  const int b = (int)(top >> 23) - 2 + ((rule == kMx4NoClip && (top & 0x7FFFFFu) > 0x400000u) ? 1 : 0);
+  return b < 1 ? 1 : (b > 252 ? 252 : b);
+}
+__device__ __forceinline__ float inverse_scale(int byte) { return __uint_as_float((uint32_t)(254 - byte) << 23); }
+
+// max over the four lanes of a block
+__device__ __forceinline__ uint32_t block_max(uint32_t v) {
+  v = max(v, __shfl_xor_sync(0xFFFFFFFFu, v, 1));
+  return max(v, __shfl_xor_sync(0xFFFFFFFFu, v, 2));
+}
+
+__device__ __forceinline__ uint32_t quantize8(const float (&v)[8], int rule, int *byte) {
+  uint32_t top = 0u;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(v[i]) & 0x7FFFFFFFu);
+  top = block_max(top);
+  if (top >= 0x7F800000u) {
+    *byte = 255;
+    return 0u;
+  }
+  *byte = scale_byte(top, rule);
+  return pack_scaled(v, inverse_scale(*byte));
+}
+
+// The clamped SwiGLU in f64, correct to far below an f32 rounding.
+__device__ __forceinline__ double swiglu_f64(float gf, float uf, float alpha, float limit) {
+  const double g = gf > limit ? limit : gf, u = uf < -limit ? -limit : (uf > limit ? limit : uf);
+  return g * (1.0 / (1.0 + exp(-(double)alpha * g))) * (u + 1.0);
+}
+
+// Eight SwiGLU outputs from their gate / up pairs, quantised as the exact values would be. The f32 value is
+// within (|alpha g| + 9) 2^-24 of the exact one, relatively: one rounding of alpha g, which the exponential
+// turns into |alpha g| 2^-24; at most 2 ulp of expf; the roundings of the sum, the quotient, u + 1 and two
+// products. While -alpha g <= 80 that is below kTol = 2^-17. So where the block's largest magnitude or a
+// scaled element lies within kTol of a border between two scales or two codes (seen by rounding both
+// (1 - kTol) and (1 + kTol) times the value), where alpha g < -80, or where a product has left the
+// range in which f32 is that exact, the block's four lanes evaluate it again in f64: about 1 block in 300
+// of normally distributed inputs, so codes do not depend on which exponential computed them.
+constexpr float kTol = 0x1p-17f;
+__device__ __forceinline__ uint32_t swiglu_quantize8_f64(const float (&gu)[16], float alpha, float limit, int rule, int *byte,
+                                                      uint32_t lanes) {
+  double h[8], top = 0.0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    h[i] = swiglu_f64(gu[2 * i], gu[2 * i + 1], alpha, limit);
+    top = fabs(h[i]) > top ? fabs(h[i]) : top;
+  }
+#pragma unroll
+  for (int o = 1; o <= 2; o <<= 1) {
+    const double other = __shfl_xor_sync(lanes, top, o);
+    top = other > top ? other : top;
+  }
+  const long long bits = __double_as_longlong(top);
+  int b = (int)(bits >> 52) - 1023 + 127 - 2;
+  if (rule == kMx4NoClip && (bits & 0xFFFFFFFFFFFFFll) > 0x8000000000000ll) b += 1;
+  *byte = b = b < 1 ? 1 : (b > 252 ? 252 : b);
+  uint32_t w = 0u;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const double r = scalbn(fabs(h[i]), 127 - b);
+    const uint32_t c = (r > 0.25) + (r >= 0.75) + (r > 1.25) + (r >= 1.75) + (r > 2.5) + (r >= 3.5) + (r > 5.0);
+    w |= (c | (signbit(h[i]) ? 8u : 0u)) << (4 * i);
+  }
+  return w;
+}
+__device__ __forceinline__ uint32_t swiglu_quantize8(const float (&gu)[16], float alpha, float limit, int rule, int *byte) {
+  float h[8];
+  uint32_t top = 0u;
+  bool close = false;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    float g = gu[2 * i], u = gu[2 * i + 1];
+    g = g > limit ? limit : g;
+    u = u < -limit ? -limit : (u > limit ? limit : u);
+    const float x = -alpha * g, up = u + 1.0f;
+    h[i] = g * (1.0f / (1.0f + expf(x))) * up;
+    close |= x > 80.f || (fabsf(h[i]) < 0x1p-100f && g != 0.f && up != 0.f);
+    top = max(top, __float_as_uint(h[i]) & 0x7FFFFFFFu);
+  }
+  top = block_max(top);
+  const bool finite = top < 0x7F800000u;
+  const float t = __uint_as_float(top);
+  *byte = finite ? scale_byte(top, rule) : 255;
+  const float inv = inverse_scale(finite ? *byte : 1);
+  const uint32_t w = pack_scaled(h, inv * (1.0f - kTol)), w1 = pack_scaled(h, inv * (1.0f + kTol));
+  close |= w != w1 || scale_byte(__float_as_uint(t * (1.0f - kTol)), rule) != scale_byte(__float_as_uint(t * (1.0f + kTol)), rule);
+  const int lane = threadIdx.x & 31;
+  const uint32_t lanes = 0xFu << (lane & ~3);
+  if (((__ballot_sync(0xFFFFFFFFu, close && finite) & lanes) != 0u))  // the four lanes of a block go together
+    return swiglu_quantize8_f64(gu, alpha, limit, rule, byte, lanes);
+  return finite ? w : 0u;
+}
+
+template <int T, bool SWIGLU, bool VEC, int UNR>
+__global__ void __launch_bounds__(kThreads) mx4_quantize_kernel(const Mx4QuantArgs a, size_t n_chunks) {
+  constexpr int N = SWIGLU ? 16 : 8;
+  const uint32_t per_row = (uint32_t)(a.cols / 8);
+  const size_t stride = (size_t)gridDim.x * kThreads;
+  // every lane of a warp makes the same rounds (shuffles below); chunks come in fours, so blocks stay whole
+  for (size_t c0 = (size_t)blockIdx.x * kThreads + threadIdx.x; c0 - (threadIdx.x & 31) < n_chunks; c0 += UNR * stride) {
+    Raw<T, N, VEC> raw[UNR];
+    size_t row[UNR];
+    uint32_t col[UNR];
+#pragma unroll
+    for (int u = 0; u < UNR; ++u) {
+      const size_t c = c0 + u * stride;
+      if (n_chunks <= 0xFFFFFFFFull) {
+        row[u] = (uint32_t)c / per_row;
+        col[u] = (uint32_t)c - (uint32_t)row[u] * per_row;
+      } else {
+        row[u] = c / per_row;
+        col[u] = (uint32_t)(c - row[u] * per_row);
+      }
+      if (c < n_chunks)
+        raw[u].load(static_cast<const uint8_t *>(a.x) + (row[u] * a.ld + (size_t)col[u] * N) * Elem<T>::kBytes);
+      else
+#pragma unroll
+        for (int i = 0; i < Raw<T, N, VEC>::kWords; ++i) raw[u].w[i] = make_uint4(0u, 0u, 0u, 0u);
+    }
+#pragma unroll
+    for (int u = 0; u < UNR; ++u) {
+      const size_t c = c0 + u * stride;
+      float v[N];
+      raw[u].values(v);
+      int byte;
+      uint32_t w;
+      if constexpr (SWIGLU) {
+        w = swiglu_quantize8(v, a.alpha, a.limit, a.rule, &byte);
+      } else {
+        if (a.row_scale) {
+          const float f = c < n_chunks ? __ldg(a.row_scale + row[u]) : 0.f;
+#pragma unroll
+          for (int i = 0; i < N; ++i) v[i] = __fmul_rn(v[i], f);
+        }
+        w = quantize8(v, a.rule, &byte);
+      }
+      if (c >= n_chunks) continue;
+      reinterpret_cast<uint32_t *>(a.blocks)[c] = w;
+      if ((c & 3) == 0) {
+        if (!a.tiled) {
+          a.scales[c >> 2] = (uint8_t)byte;
+        } else {
+          const uint32_t kb = col[u] >> 2;
+          uint8_t *d = a.scales + ((size_t)(kb >> 2) * a.rows + row[u]) * 4;
+          d[kb & 3] = (uint8_t)byte;
+          if (col[u] + 4 == per_row)  // zero where the row ends inside a 128-element stretch
+            for (uint32_t j = (kb & 3) + 1; j < 4; ++j) d[j] = 0;
+        }
+      }
+    }
+  }
+}
+
+// One thread per 4-byte word, consecutive rows side by side in the output.
+__global__ void __launch_bounds__(kThreads)
+    mx4_tile_scales_kernel(const uint8_t *__restrict__ src, size_t n_words, size_t rows, uint32_t kb, uint32_t words,
+                           uint32_t *__restrict__ dst) {
+  for (size_t i = (size_t)blockIdx.x * kThreads + threadIdx.x; i < n_words; i += (size_t)gridDim.x * kThreads) {
+    const size_t r = i % rows, q = i / rows, g = q / words;
+    const uint32_t b0 = (uint32_t)(q - g * words) * 4;
+    const uint8_t *s = src + (g * rows + r) * kb + b0;
+    uint32_t w = 0u;
+#pragma unroll
+    for (uint32_t j = 0; j < 4; ++j)
+      if (b0 + j < kb) w |= (uint32_t)__ldg(s + j) << (8 * j);
+    dst[i] = w;
+  }
+}
+
+template <int T, bool SWIGLU, bool VEC>
+cudaError_t launch_quant(const Mx4QuantArgs &a, int n_sms, cudaStream_t stream) {
+  constexpr int UNR = 1;
+  const size_t n_chunks = a.rows * (a.cols / 8);
+  const size_t want = (n_chunks + (size_t)kThreads * UNR - 1) / ((size_t)kThreads * UNR), cap = (size_t)n_sms * 8;
+  mx4_quantize_kernel<T, SWIGLU, VEC, UNR><<<(unsigned)(want < cap ? want : cap), kThreads, 0, stream>>>(a, n_chunks);
+  return cudaGetLastError();
+}
+template <int T>
+cudaError_t launch_typed(const Mx4QuantArgs &a, bool swiglu, int n_sms, cudaStream_t stream) {
+  const bool vec = (uintptr_t)a.x % 16 == 0 && a.ld * Elem<T>::kBytes % 16 == 0;
+  if (swiglu) return vec ? launch_quant<T, true, true>(a, n_sms, stream) : launch_quant<T, true, false>(a, n_sms, stream);
+  return vec ? launch_quant<T, false, true>(a, n_sms, stream) : launch_quant<T, false, false>(a, n_sms, stream);
+}
+
+}  // namespace
+
+cudaError_t launch_mx4_quantize(const Mx4QuantArgs &a, int dtype, bool swiglu, int n_sms, cudaStream_t stream) {
+  if (a.rows == 0 || a.cols == 0) return cudaSuccess;
+  if (dtype == kMx4F32) return launch_typed<kMx4F32>(a, swiglu, n_sms, stream);
+  if (dtype == kMx4Bf16) return launch_typed<kMx4Bf16>(a, swiglu, n_sms, stream);
+  return launch_typed<kMx4F16>(a, swiglu, n_sms, stream);
+}
+
+cudaError_t launch_mx4_tile_scales(const uint8_t *src, size_t groups, size_t rows, size_t cols, uint8_t *dst, int n_sms,
+                                   cudaStream_t stream) {
+  const uint32_t kb = (uint32_t)(cols / 32), words = (kb + 3) / 4;
+  const size_t n_words = groups * rows * words;
+  if (n_words == 0) return cudaSuccess;
+  const size_t want = (n_words + kThreads - 1) / kThreads, cap = (size_t)n_sms * 16;
+  mx4_tile_scales_kernel<<<(unsigned)(want < cap ? want : cap), kThreads, 0, stream>>>(src, n_words, rows, kb, words,
+                                                                                       reinterpret_cast<uint32_t *>(dst));
+  return cudaGetLastError();
+}
+
+}  // namespace oxg

@@ -61,6 +61,24 @@ __device__ __forceinline__ void umma_mxf(uint32_t d_tmem, uint64_t a_desc, uint6
       : "memory");
 }
 
+// kind::mxf4: A and B packed E2M1 (two codes in a byte; K = 64 takes 32 bytes of a row), both K-major,
+// UE8M0 scales for 32 elements each, so one MMA takes two of an atom's four scale columns: sf = 0 or 2.
+__host__ __device__ constexpr uint32_t idesc_mxf4(int m, int n, int sf) {
+  return ((uint32_t)sf << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(n >> 3) << 17) | (1u << 23) |
+         ((uint32_t)(m >> 4) << 24) | ((uint32_t)sf << 29);
+}
+
+__device__ __forceinline__ void umma_mxf4(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
+                                          uint32_t sfa_tmem, uint32_t sfb_tmem, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.block32 [%0], %1, %2, %3, [%5], [%6], p;\n\t}" ::"r"(
+          d_tmem),
+      "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate), "r"(sfa_tmem), "r"(sfb_tmem)
+      : "memory");
+}
+
 // Copies a 512-byte scale atom from shared memory into 4 TMEM columns of all
 // four lane quarters. Ordered with the MMAs the same thread issues.
 __device__ __forceinline__ void utccp_atom(uint32_t taddr, uint32_t atom_saddr) {

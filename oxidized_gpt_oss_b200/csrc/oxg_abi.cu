@@ -157,6 +157,8 @@ struct oxg_ctx {
   bool prefill_pending = false;  // a prefill ran since the error word was last read
   Profiler prof;
   oxg::ModelState *model = nullptr;  // full-model state (model_abi.cu)
+  int *op_err = nullptr;         // error word of the MXFP4 products (mx4_abi.cu)
+  bool op_used = false;          // one of them has run
   unsigned long long epoch = 0;  // bumped when uploaded layers or the scratch move
   // Expert-parallel receive side (oxg_moe_experts): kept apart from ws so
   // that sizing it for the received rows never discards the dispatch's
@@ -872,6 +874,10 @@ int ctx_error(oxg_ctx *ctx, int status, const char *msg) { return fail(ctx, stat
 int ctx_device(const oxg_ctx *ctx) { return ctx->device; }
 cudaStream_t ctx_stream(const oxg_ctx *ctx) { return ctx->stream; }
 int ctx_n_sms(const oxg_ctx *ctx) { return ctx->n_sms; }
+int *ctx_op_err(oxg_ctx *ctx) {
+  ctx->op_used = true;
+  return ctx->op_err;
+}
 
 int ctx_moe_forward(oxg_ctx *ctx, int layer, const uint16_t *x, int T, float *y) {
   return oxg_moe_forward(ctx, layer, x, T, y, OXG_MODE_AUTO, OXG_PRECISION_PARITY);
@@ -975,6 +981,13 @@ int oxg_ctx_create(int device, oxg_ctx **out) {
     return cuda_fail(nullptr, st, "cudaStreamCreate");
   }
   ctx->stream = ctx->own_stream;
+  if ((st = cudaMalloc((void **)&ctx->op_err, sizeof(int))) == cudaSuccess) st = cudaMemset(ctx->op_err, 0, sizeof(int));
+  if (st != cudaSuccess) {
+    if (ctx->op_err) cudaFree(ctx->op_err);
+    cudaStreamDestroy(ctx->own_stream);
+    delete ctx;
+    return cuda_fail(nullptr, st, "cudaMalloc(error word)");
+  }
   *out = ctx;
   return OXG_OK;
 }
@@ -988,6 +1001,7 @@ int oxg_ctx_destroy(oxg_ctx *ctx) {
   if (ctx->ws.base) cudaFree(ctx->ws.base);
   if (ctx->comb_cnt) cudaFree(ctx->comb_cnt);
   if (ctx->ep.base) cudaFree(ctx->ep.base);
+  if (ctx->op_err) cudaFree(ctx->op_err);
   if (ctx->pipe.h2d) cudaStreamSynchronize(ctx->pipe.h2d);
   if (ctx->pipe.d2h) cudaStreamSynchronize(ctx->pipe.d2h);
   for (int b = 0; b < 2; ++b) {
@@ -1022,8 +1036,9 @@ int oxg_sync(oxg_ctx *ctx) {
   if (!ctx) return fail(nullptr, OXG_ERR_INVALID_ARG, "ctx is NULL");
   DeviceGuard g(ctx->device);
   OXG_CUDA(ctx, cudaStreamSynchronize(ctx->stream), "cudaStreamSynchronize");
-  const int rc = read_pipeline_error(ctx);
+  int rc = read_pipeline_error(ctx);
   if (rc) return rc;
+  if ((rc = oxg::mx4_check_error(ctx, ctx->op_used ? ctx->op_err : nullptr))) return rc;
   return oxg::model_check_error(ctx);
 }
 

@@ -28,23 +28,6 @@ constexpr int kPeakM = 128, kPeakN = 256;
 constexpr int kPeakA = kPeakM * 128, kPeakB = kPeakN * 128;  // bytes of the two tiles
 constexpr int kPeakErr = 31;  // error word: the final commit did not arrive
 
-// kind::mxf4 instruction descriptor: A and B E2M1 (format 1 of this kind),
-// UE8M0 scales, K-major, dense K = 64.
-__host__ __device__ constexpr uint32_t idesc_mxf4(int m, int n) {
-  return (1u << 7) | (1u << 10) | ((uint32_t)(n >> 3) << 17) | (1u << 23) | ((uint32_t)(m >> 4) << 24);
-}
-
-__device__ __forceinline__ void umma_mxf4(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
-                                          uint32_t sfa_tmem, uint32_t sfb_tmem, uint32_t accumulate) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.block32 [%0], %1, %2, %3, [%5], [%6], p;\n\t}" ::"r"(
-          d_tmem),
-      "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate), "r"(sfa_tmem), "r"(sfb_tmem)
-      : "memory");
-}
-
 template <int KIND>
 __global__ void __launch_bounds__(128, 1) mma_rate_kernel(int iters, int *err) {
   extern __shared__ uint8_t peak_raw[];
@@ -82,7 +65,7 @@ __global__ void __launch_bounds__(128, 1) mma_rate_kernel(int iters, int *err) {
       else if (KIND == 1)
         mxf::umma_mxf(tmem, ad + 2 * kk, bd + 2 * kk, mxf::idesc_e2m1_e4m3(kPeakM, kPeakN, 0, 0), sfa, sfb, i != 0);
       else
-        umma_mxf4(tmem, ad + 2 * kk, bd + 2 * kk, idesc_mxf4(kPeakM, kPeakN), sfa, sfb, i != 0);
+        mxf::umma_mxf4(tmem, ad + 2 * kk, bd + 2 * kk, mxf::idesc_mxf4(kPeakM, kPeakN, 0), sfa, sfb, i != 0);
     }
     umma_commit(&done_bar);
     mbar_wait(&done_bar, 0, err, kPeakErr);

@@ -10,7 +10,7 @@ from __future__ import annotations
 import torch
 
 from . import abi
-from .mxfp4 import context
+from .mxfp4 import _DTYPES, check_status, context, device_context, quantized_like, rows_of, scale_rule_code
 
 ALPHA = 1.702
 LIMIT = 7.0
@@ -29,3 +29,22 @@ def swiglu(gate: torch.Tensor, up: torch.Tensor, alpha: float = ALPHA, limit: fl
     abi.check(c.lib.oxg_swiglu(c.handle, g.data_ptr(), u.data_ptr(), g.numel(), float(alpha), float(limit),
                                out.data_ptr()), c.handle)
     return out
+
+
+def swiglu_quantize_mxfp4(gate_up: torch.Tensor, alpha: float = ALPHA, limit: float = LIMIT, *,
+                          scale_rule: str = "floor", tiled: bool = False,
+                          ctx: abi.Context | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """The clamped SwiGLU of gate_up [..., 2 cols] (gate in the even columns, up
+    in the odd ones, as the experts' first product gives them; float32, bfloat16
+    or float16), as MXFP4 [..., cols]: (blocks, scales) as
+    ``mxfp4.quantize_mxfp4`` returns them, with the codes of the exact values."""
+    x2, rows, ld = rows_of(gate_up, "gate_up")
+    if gate_up.shape[-1] % 2:
+        raise ValueError(f"gate_up must hold pairs, got {gate_up.shape[-1]} columns")
+    cols = gate_up.shape[-1] // 2
+    blocks, scales = quantized_like(gate_up, cols, rows, tiled)
+    c = device_context(gate_up, ctx)
+    check_status(c.lib.oxg_swiglu_quantize_mxfp4(c.handle, x2.data_ptr(), _DTYPES[gate_up.dtype], rows, cols, ld,
+                                                 float(alpha), float(limit), scale_rule_code(scale_rule), int(tiled),
+                                                 blocks.data_ptr(), scales.data_ptr()), c)
+    return blocks, scales

@@ -6,6 +6,15 @@ signature and meaning (src/mxfp4.rs:15): ``blocks`` are packed E2M1 codes
 ``rows * cols`` bf16 bit patterns. Inputs are CUDA tensors; the work runs in
 liboxg_b200.so on torch's current stream. Shape violations raise
 ``ValueError`` with the reference's assert text where the reference panics.
+
+The way back and what 4-bit operands are for (no counterpart in the reference):
+``quantize_mxfp4`` makes blocks and scales of floating-point rows,
+``mxfp4_matmul`` multiplies two MXFP4 operands on the 4-bit tensor cores, and
+``mxfp4_grouped_matmul`` does so for runs of rows that each have a matrix of
+their own (experts). The products read scales in the tiled layout
+``[ceil(k / 128), rows, 4]``, which the quantisers write with ``tiled=True`` and
+``tile_scales`` makes of a checkpoint's ``[rows, k / 32]``; given the latter,
+they convert it first, on every call.
 """
 from __future__ import annotations
 
@@ -51,4 +60,194 @@ def dequantize_mxfp4(blocks: torch.Tensor, scales: torch.Tensor, rows: int, cols
     if st == abi.OXG_ERR_SHAPE:
         raise ValueError(c.lib.oxg_last_error(c.handle).decode())
     abi.check(st, c.handle)
+    return out
+
+
+_DTYPES = {torch.float32: abi.OXG_DTYPE_F32, torch.bfloat16: abi.OXG_DTYPE_BF16, torch.float16: abi.OXG_DTYPE_F16}
+_RULES = {"floor": abi.OXG_MX_FLOOR, "noclip": abi.OXG_MX_NOCLIP}
+_device_ctx: dict[int, abi.Context] = {}
+
+
+def device_context(x: torch.Tensor, ctx: abi.Context | None) -> abi.Context:
+    """The given context, or a per-process one on x's device, bound to torch's
+    current stream there."""
+    index = x.device.index
+    if ctx is None:
+        ctx = _default_ctx if _default_ctx is not None and _default_ctx.device == index else _device_ctx.get(index)
+        if ctx is None:
+            ctx = _device_ctx[index] = abi.Context(index)
+    elif ctx.device != index:
+        raise ValueError(f"the context is on cuda:{ctx.device}, the input on {x.device}")
+    ctx.set_stream(torch.cuda.current_stream(index))
+    return ctx
+
+
+def check_status(status: int, ctx: abi.Context) -> None:
+    """ValueError where the library refuses shapes or arguments, OxgError else."""
+    if status in (abi.OXG_ERR_SHAPE, abi.OXG_ERR_INVALID_ARG):
+        raise ValueError(ctx.lib.oxg_last_error(ctx.handle).decode())
+    abi.check(status, ctx.handle)
+
+
+def rows_of(x: torch.Tensor, name: str) -> tuple[torch.Tensor, int, int]:
+    """x [..., width] as a 2-D view (a copy only where its rows have no common
+    pitch or are not contiguous) with its row count and pitch in elements."""
+    if not x.is_cuda or x.dtype not in _DTYPES:
+        raise ValueError(f"{name} must be a float32, bfloat16 or float16 CUDA tensor")
+    if x.dim() == 0:
+        raise ValueError(f"{name} must have at least one dimension")
+    if x.dim() != 2:
+        x = x.reshape(-1, x.shape[-1]) if x.shape[-1] else x.reshape(0, 0)
+    if x.shape[1] > 1 and x.stride(1) != 1 or x.shape[0] > 1 and x.stride(0) < x.shape[1]:
+        x = x.contiguous()
+    return x, x.shape[0], x.stride(0) if x.shape[0] > 1 else x.shape[1]
+
+
+def scale_rule_code(rule: str) -> int:
+    if rule not in _RULES:
+        raise ValueError(f"unknown scale rule {rule!r}: one of {', '.join(_RULES)}")
+    return _RULES[rule]
+
+
+def quantized_like(x: torch.Tensor, cols: int, rows: int, tiled: bool) -> tuple[torch.Tensor, torch.Tensor]:
+    """Empty blocks and scales for the MXFP4 form of x's rows at `cols` columns."""
+    if cols % 32:
+        raise ValueError(f"cols must be divisible by 32, got {cols}")
+    if tiled and x.dim() != 2:
+        raise ValueError(f"tiled scales are those of one matrix: the input must have 2 dimensions, got {x.dim()}")
+    lead = x.shape[:-1]
+    blocks = torch.empty(*lead, cols // 2, dtype=torch.uint8, device=x.device)
+    shape = ((cols + 127) // 128, rows, 4) if tiled else (*lead, cols // 32)
+    return blocks, torch.empty(shape, dtype=torch.uint8, device=x.device)
+
+
+def quantize_mxfp4(x: torch.Tensor, *, row_scale: torch.Tensor | None = None, scale_rule: str = "floor",
+                   tiled: bool = False, ctx: abi.Context | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """x [..., cols] (float32, bfloat16 or float16 CUDA tensor, cols a multiple
+    of 32) -> (blocks [..., cols / 2] uint8, scales [..., cols / 32] uint8), the
+    nearest E2M1 codes under a power-of-two scale for each 32 elements.
+
+    row_scale: float32 factor for each row, applied first. scale_rule: "floor"
+    (the largest element of a block lands in [4, 8) and what is above 6 becomes
+    6) or "noclip" (it lands in (3, 6]). tiled: scales as the products read
+    them, [ceil(cols / 128), rows, 4] (x must be a matrix). A block that holds an
+    infinity or a NaN reads as NaN."""
+    x2, rows, ld = rows_of(x, "x")
+    cols = x.shape[-1]
+    blocks, scales = quantized_like(x, cols, rows, tiled)
+    if row_scale is not None:
+        if row_scale.dtype != torch.float32 or row_scale.numel() != rows or row_scale.device != x.device:
+            raise ValueError(f"row_scale must be {rows} float32 values on {x.device}")
+        row_scale = row_scale.contiguous()
+    c = device_context(x, ctx)
+    check_status(c.lib.oxg_quantize_mxfp4(c.handle, x2.data_ptr(), _DTYPES[x.dtype], rows, cols, ld,
+                                          None if row_scale is None else row_scale.data_ptr(),
+                                          scale_rule_code(scale_rule), int(tiled), blocks.data_ptr(),
+                                          scales.data_ptr()), c)
+    return blocks, scales
+
+
+def tile_scales(scales: torch.Tensor, *, ctx: abi.Context | None = None) -> torch.Tensor:
+    """Scales [..., rows, k / 32] uint8 as the products read them:
+    [..., ceil(k / 128), rows, 4], zero where k ends inside a 128-element stretch."""
+    if not scales.is_cuda or scales.dtype != torch.uint8 or scales.dim() < 2:
+        raise ValueError("scales must be a uint8 CUDA tensor [..., rows, k / 32]")
+    scales = scales.contiguous()
+    *lead, rows, kb = scales.shape
+    out = torch.empty(*lead, (kb + 3) // 4, rows, 4, dtype=torch.uint8, device=scales.device)
+    c = device_context(scales, ctx)
+    groups = 1
+    for n in lead:
+        groups *= n
+    check_status(c.lib.oxg_mxfp4_tile_scales(c.handle, scales.data_ptr(), groups, rows, 32 * kb, out.data_ptr()), c)
+    return out
+
+
+def _operand(blocks: torch.Tensor, scales: torch.Tensor, name: str, dim: int, device,
+             ctx: abi.Context | None) -> tuple[torch.Tensor, torch.Tensor]:
+    """One operand's blocks and tiled scales, contiguous, checked against each other."""
+    if blocks.dtype != torch.uint8 or scales.dtype != torch.uint8 or not blocks.is_cuda or \
+            blocks.device != device or scales.device != device:
+        raise ValueError(f"{name}'s blocks and scales must be uint8 tensors on one CUDA device with the other operand")
+    if blocks.dim() != dim:
+        raise ValueError(f"{name}'s blocks must have {dim} dimensions, got {tuple(blocks.shape)}")
+    *lead, rows, half = blocks.shape
+    k = 2 * half
+    if k == 0 or k % 32:
+        raise ValueError(f"k must be a positive multiple of 32, got {k}")
+    if scales.dim() == dim and tuple(scales.shape) == (*lead, rows, k // 32):
+        scales = tile_scales(scales, ctx=ctx)
+    elif tuple(scales.shape) != (*lead, (k + 127) // 128, rows, 4):
+        raise ValueError(f"{name}'s scales must be {(*lead, (k + 127) // 128, rows, 4)} (tiled) or {(*lead, rows, k // 32)}, "
+                         f"got {tuple(scales.shape)}")
+    return blocks.contiguous(), scales.contiguous()
+
+
+def _output(out: torch.Tensor | None, out_dtype: torch.dtype, m: int, n: int, device) -> tuple[torch.Tensor, int, int]:
+    """The output tensor, its type's code and its row pitch."""
+    if out is None:
+        if out_dtype not in (torch.float32, torch.bfloat16):
+            raise ValueError(f"out_dtype must be float32 or bfloat16, got {out_dtype}")
+        out = torch.empty(m, n, dtype=out_dtype, device=device)
+    elif tuple(out.shape) != (m, n) or out.dtype not in (torch.float32, torch.bfloat16) or out.device != device or \
+            (n > 1 and out.stride(1) != 1) or (m > 1 and out.stride(0) < n):
+        raise ValueError(f"out must be a float32 or bfloat16 [{m}, {n}] on {device} with contiguous rows")
+    return out, _DTYPES[out.dtype], out.stride(0) if m > 1 else n
+
+
+def _bias(bias: torch.Tensor | None, shape: tuple, device) -> torch.Tensor | None:
+    if bias is None:
+        return None
+    if bias.dtype != torch.bfloat16 or tuple(bias.shape) != shape or bias.device != device:
+        raise ValueError(f"bias must be bfloat16 {shape} on {device}, got {bias.dtype} {tuple(bias.shape)}")
+    return bias.contiguous()
+
+
+def mxfp4_matmul(a_blocks: torch.Tensor, a_scales: torch.Tensor, b_blocks: torch.Tensor, b_scales: torch.Tensor, *,
+                 bias: torch.Tensor | None = None, out_dtype: torch.dtype = torch.bfloat16,
+                 out: torch.Tensor | None = None, ctx: abi.Context | None = None) -> torch.Tensor:
+    """a [m, k] times b [n, k] transposed, plus ``bias`` [n] (bfloat16), both
+    operands MXFP4 (blocks [rows, k / 2], scales tiled [ceil(k / 128), rows, 4] or
+    [rows, k / 32]); f32 sums, returned as ``out_dtype`` (float32 or bfloat16)."""
+    device = a_blocks.device
+    a_blocks, a_scales = _operand(a_blocks, a_scales, "a", 2, device, ctx)
+    b_blocks, b_scales = _operand(b_blocks, b_scales, "b", 2, device, ctx)
+    m, n, k = a_blocks.shape[0], b_blocks.shape[0], 2 * a_blocks.shape[1]
+    if 2 * b_blocks.shape[1] != k:
+        raise ValueError(f"a has rows of {k} elements, b of {2 * b_blocks.shape[1]}")
+    out, code, ldo = _output(out, out_dtype, m, n, device)
+    bias = _bias(bias, (n,), device)
+    c = device_context(a_blocks, ctx)
+    check_status(c.lib.oxg_mxfp4_matmul(c.handle, a_blocks.data_ptr(), a_scales.data_ptr(), m, b_blocks.data_ptr(),
+                                        b_scales.data_ptr(), n, k, None if bias is None else bias.data_ptr(),
+                                        out.data_ptr(), code, ldo), c)
+    return out
+
+
+def mxfp4_grouped_matmul(a_blocks: torch.Tensor, a_scales: torch.Tensor, counts: torch.Tensor, b_blocks: torch.Tensor,
+                         b_scales: torch.Tensor, *, bias: torch.Tensor | None = None,
+                         out_dtype: torch.dtype = torch.bfloat16, out: torch.Tensor | None = None,
+                         ctx: abi.Context | None = None) -> torch.Tensor:
+    """Runs of a's rows, each times a matrix of its own: the first counts[0] rows
+    of a [m, k] times b[0] [n, k] transposed, the next counts[1] times b[1] and so
+    on (counts: int32 CUDA tensor, zeros allowed; ``MoELayer.dispatch`` returns
+    them). bias [groups, n] bfloat16. Rows past the last group keep what ``out``
+    held (nothing in particular in a new one). Counts that are negative or add
+    up to more than m are reported by the context's next ``sync``."""
+    device = a_blocks.device
+    a_blocks, a_scales = _operand(a_blocks, a_scales, "a", 2, device, ctx)
+    b_blocks, b_scales = _operand(b_blocks, b_scales, "b", 3, device, ctx)
+    m, k = a_blocks.shape[0], 2 * a_blocks.shape[1]
+    groups, n = b_blocks.shape[:2]
+    if 2 * b_blocks.shape[2] != k:
+        raise ValueError(f"a has rows of {k} elements, b of {2 * b_blocks.shape[2]}")
+    if counts.dtype != torch.int32 or tuple(counts.shape) != (groups,) or counts.device != device:
+        raise ValueError(f"counts must be int32 [{groups}] on {device}, got {counts.dtype} {tuple(counts.shape)}")
+    counts = counts.contiguous()
+    out, code, ldo = _output(out, out_dtype, m, n, device)
+    bias = _bias(bias, (groups, n), device)
+    c = device_context(a_blocks, ctx)
+    check_status(c.lib.oxg_mxfp4_grouped_matmul(c.handle, a_blocks.data_ptr(), a_scales.data_ptr(), m, counts.data_ptr(),
+                                                groups, b_blocks.data_ptr(), b_scales.data_ptr(), n, k,
+                                                None if bias is None else bias.data_ptr(), out.data_ptr(), code, ldo), c)
     return out
