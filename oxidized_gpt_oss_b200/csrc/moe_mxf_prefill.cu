@@ -86,14 +86,6 @@ struct StageX {
   static constexpr uint32_t TX_PAIR = 2u * (A + kBTx + SFA + SFB);
 };
 
-__device__ __forceinline__ void utccp_atom_pair(uint32_t taddr, uint32_t atom_saddr) {
-  uint64_t d = 0;
-  d |= (uint64_t)((atom_saddr >> 4) & 0x3FFFu);
-  d |= (uint64_t)1 << 16;
-  d |= (uint64_t)(128 >> 4) << 32;
-  d |= (uint64_t)1 << 46;
-  asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(d) : "memory");
-}
 __device__ __forceinline__ void umma_mxf_pair(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
                                               uint32_t sfa_tmem, uint32_t sfb_tmem, uint32_t accumulate) {
   asm volatile(

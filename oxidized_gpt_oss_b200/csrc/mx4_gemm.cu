@@ -5,23 +5,30 @@
 // and adds up in f32 in tensor memory; a scale byte of 255 makes the sums that it takes part in NaN, 0 stands
 // for 2^-127.
 //
-// The weight rows are the MMA's M side (128 a tile), the activation rows its N side (up to kTileN a tile,
-// in steps of 16: a group's rows are cut into equal tiles, so a short group costs a short tile and one row
-// costs 16). A TMEM lane then is one feature, and a warp's stores of a column are 32 consecutive features of
-// one output row.
+// The weight rows are the MMA's M side (128 per CTA), the activation rows its N side: a group's rows are cut
+// into equal tiles, so a short group costs a short tile. A TMEM lane then is one feature, and a warp's stores
+// of a column are 32 consecutive features of one output row.
 //
 // Scales come in words of four (one 128-element stretch of a row), the words of consecutive rows side by
-// side, so that a group may start at any row: a warp's 32 lanes fetch 32 rows' words with one coalesced
-// 4-byte cp.async each and drop them where the tensor core's 512-byte atom (128 rows x 4 blocks, row r at
-// 16 (r % 32) + 4 (r / 32)) wants them.
+// side, so that a group may start at any row: lane l of a warp loads the words of rows l, l + 32, l + 64 and
+// l + 96 (each load coalesced) and stores them as the 16 bytes that the tensor core's scale atom (128 rows x
+// 4 blocks, row r at 16 (r % 32) + 4 (r / 32)) has for it.
 //
-// One CTA per SM walks its tiles (weight tile fastest, so CTAs side by side share activation rows and a
-// group's weights stay in L2). Warps: 0 TMA (codes, 128-byte swizzle), 1 MMA, 2 scales, 3 idle, 4-7
-// epilogue (two accumulators, so it drains one tile while the next is computed).
+// Two kernels share this code. For many rows, pairs of CTAs (cta_group::2) work on 256 weight rows x up to 224
+// activation rows, so that each SM fetches and reads half of the activation codes. For few rows, a CTA
+// works on 128 weight rows x up to 64 activation rows, with more stages of weight codes in flight, and where
+// there are fewer tiles than SMs, a cluster splits a tile's K and adds the parts through distributed shared
+// memory in rank order (so a result does not depend on timing).
+//
+// CTAs walk their tiles with the weight tile fastest: CTAs side by side share activation rows, and a group's
+// weights stay in L2. Warps: 0 TMA (codes, 128-byte swizzle), 1 MMA, 2-3 and 8-9 scales (weights and
+// activations, each stage's by one of two warps, which fetches its next stage's words before it waits for
+// that stage's memory), 4-7 epilogue (two accumulators: one tile drains while the next is computed).
 // Every wait is bounded; one that runs out sets the error word and the CTA winds down.
 #include <cuda.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "common.cuh"
 #include "mx4.h"
@@ -33,21 +40,30 @@ namespace {
 using namespace sm100;
 using namespace mxf;
 
-constexpr int kTileW = 128;                      // weight rows per tile
-constexpr int kTileN = 224;                      // most activation rows per tile
-constexpr int kStageK = 256;                     // elements of K per stage: 128 bytes of codes
-constexpr int kBoxN = 32;                        // activation rows per TMA box
-constexpr int kWBytes = kTileW * 128;            // a stage's weight codes
-constexpr int kXBytes = kTileN * 128;            // a stage's activation codes
-constexpr int kSfw = 2 * kAtomBytes;             // two words of K for 128 weight rows
-constexpr int kSfx = 4 * kAtomBytes;             // two words for each 128 activation rows
-constexpr int kStageBytes = kWBytes + kXBytes + kSfw + kSfx;
-constexpr int kStages = 4;
-constexpr int kThreads = 256;
+constexpr int kTileW = 128;           // weight rows per CTA
+constexpr int kStageK = 256;          // elements of K per stage: 128 bytes of codes
+constexpr int kThreads = 320;
 constexpr int kEpiWarps = 4;
-constexpr uint32_t kTmemCols = 512;
-constexpr uint32_t kSfwCol = 2 * kTileN, kSfxCol = kSfwCol + 8;  // behind the two accumulators
-static_assert(kStageBytes % 1024 == 0 && kSfxCol + 16 <= kTmemCols, "stage and tensor-memory layout");
+constexpr int kWBytes = kTileW * 128;  // a stage's weight codes
+
+// PAIR: two CTAs per tile. NMAX: most activation rows per tile. SPLIT: a cluster per tile, K split.
+template <bool PAIR_, int NMAX_, int STAGES_, bool SPLIT_>
+struct Cfg {
+  static constexpr bool PAIR = PAIR_, SPLIT = SPLIT_;
+  static constexpr int NMAX = NMAX_, STAGES = STAGES_;
+  static constexpr int CTAS = PAIR ? 2 : 1;
+  static constexpr int X_GROUPS = (NMAX + 127) / 128;  // 128-row scale groups of the activation rows
+  static constexpr int X_BYTES = NMAX / CTAS * 128;    // a stage's activation codes in one CTA
+  static constexpr int SFW = 2 * kAtomBytes, SFX = 2 * X_GROUPS * kAtomBytes;  // two words of K each
+  static constexpr int BYTES = (kWBytes + X_BYTES + SFW + SFX + 1023) / 1024 * 1024;
+  static constexpr int SMEM = STAGES * BYTES + 1024;
+  static constexpr int SFW_COL = 2 * NMAX, SFX_COL = SFW_COL + 8;  // TMEM columns behind the two accumulators
+  static constexpr int COLS_USED = SFX_COL + 8 * X_GROUPS;
+  static constexpr uint32_t TMEM_COLS = COLS_USED <= 128 ? 128 : (COLS_USED <= 256 ? 256 : 512);
+  static_assert(COLS_USED <= 512 && X_BYTES % 1024 == 0, "tensor memory, swizzle atoms");
+  static_assert(!(PAIR && SPLIT), "a pair does not split K");
+  static_assert(!SPLIT || STAGES * BYTES >= NMAX * kTileW * 4, "the split's partial sums use the stages' memory");
+};
 
 struct Params {
   int m, n, k, groups;
@@ -56,9 +72,10 @@ struct Params {
   const uint16_t *bias;
   void *out;
   size_t ldo;
-  int n_tiles;     // weight tiles per group
-  int k_steps;     // stages per tile
-  int words;       // scale words per row
+  int n_tiles;      // weight tiles per group
+  int k_steps;      // stages per tile
+  int words;        // scale words per row
+  int box;          // activation rows per TMA box
   int out_bf16;
   int pair_stores;  // bf16 rows start on 4-byte boundaries
   int *err;
@@ -66,40 +83,122 @@ struct Params {
 
 // Where a tile lies: its group's weight rows from f0, activation rows [row0, row0 + rows).
 struct Tile {
-  int g, f0, row0, rows, cols;  // cols: rows rounded up to the MMA's 16
+  int g, f0, row0, rows, cols;  // cols: rows as the MMA's N
 };
-
-// Copies 4 bytes (or writes 0) asynchronously.
-__device__ __forceinline__ void cp_async_4_zfill(uint32_t dst, const void *src, bool ok) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(ok ? 4u : 0u) : "memory");
+// The MMA's N comes in steps of 16, a pair's of 32 (each CTA holds half of its rows).
+template <class C>
+__host__ __device__ __forceinline__ int round_cols(int rows) {
+  return (rows + 16 * C::CTAS - 1) / (16 * C::CTAS) * (16 * C::CTAS);
 }
 
+__device__ __forceinline__ void umma_mxf4_pair(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
+                                               uint32_t sfa_tmem, uint32_t sfb_tmem, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::mxf4.block_scale.block32 [%0], %1, %2, %3, [%5], [%6], p;\n\t}" ::"r"(d_tmem),
+      "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate), "r"(sfa_tmem), "r"(sfb_tmem)
+      : "memory");
+}
+__device__ __forceinline__ void tma_load_3d_pair(void *smem_dst, const void *tmap, uint32_t bar_cl, int c0, int c1, int c2) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(smem_addr(smem_dst)),
+      "l"(tmap), "r"(bar_cl), "r"(c0), "r"(c1), "r"(c2)
+      : "memory");
+}
+// Arrive on a barrier of either CTA of the pair, publishing this thread's shared-memory writes to the cluster.
+__device__ __forceinline__ void mbar_arrive_release_cluster(uint32_t bar_cl) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar_cl) : "memory");
+}
+// mbar_wait that also acquires what the other CTA of the pair released with its arrival.
+__device__ __forceinline__ bool mbar_wait_acquire_cluster(uint64_t *bar, uint32_t parity, int *err, int code) {
+  const long long t0 = clock64();
+  while (true) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2, %3;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(smem_addr(bar)), "r"(parity), "r"(1000000u)
+        : "memory");
+    if (ok) return true;
+    if (clock64() - t0 > kWaitBudgetCycles) {
+      atomicCAS(err, 0, code);
+      return false;
+    }
+  }
+}
+__device__ __forceinline__ float ld_cluster_f32(uint32_t addr_cl) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr_cl) : "memory");
+  return v;
+}
+__device__ __forceinline__ uint32_t pack_bf16x2(float lo, float hi) {
+  uint32_t r;
+  asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+
+// True in one lane of a converged warp, the same one every time. The TMA and tensor-core instructions take
+// their operands from uniform registers: issued behind elect.sync by a warp that stays together they cost a few
+// cycles each, behind `lane == 0` (where nothing tells the compiler that one lane is left) 40 to 130 (128
+// weight rows x N x 256 of K: 513 cycles a stage at N = 256 and 400 at N = 16, against 1054 at either).
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile(
+      "{\n\t.reg .pred q;\n\t"
+      "elect.sync _|q, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, q;\n\t}"
+      : "=r"(p));
+  return p != 0;
+}
+
+// A CTA's way through its tiles' stages.
+struct Cursor {
+  long long item;
+  int ks;
+  Tile t;
+};
+
+template <class C>
 __global__ void __launch_bounds__(kThreads, 1)
     mx4_gemm_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_w, const Params p) {
+  constexpr bool PAIR = C::PAIR, SPLIT = C::SPLIT;
+  constexpr int STAGES = C::STAGES;
   extern __shared__ uint8_t smem_raw[];
   uint8_t *stages = smem_raw + ((1024u - (smem_addr(smem_raw) & 1023u)) & 1023u);
-  __shared__ uint64_t full_[kStages], scaled_[kStages], empty_[kStages];
+  __shared__ uint64_t full_[STAGES], scaled_[STAGES], empty_[STAGES];
   __shared__ uint64_t acc_full[2], acc_empty[2], mma_done;
   __shared__ uint32_t tmem_slot;
   __shared__ int tile0_[kMx4MaxGroups + 1], row0_[kMx4MaxGroups + 1];
 
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xFFFFFFFFu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
+  const uint32_t rank = PAIR || SPLIT ? cluster_ctarank() : 0u;
+  uint32_t n_ranks = C::CTAS;
+  if (SPLIT) asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(n_ranks));
   if (threadIdx.x == 0) {
-    for (int s = 0; s < kStages; ++s) {
+    for (int s = 0; s < STAGES; ++s) {
       mbar_init(&full_[s], 1);
-      mbar_init(&scaled_[s], 1);
+      mbar_init(&scaled_[s], 2 * C::CTAS);
       mbar_init(&empty_[s], 1);
     }
     for (int b = 0; b < 2; ++b) {
       mbar_init(&acc_full[b], 1);
-      mbar_init(&acc_empty[b], kEpiWarps);
+      mbar_init(&acc_empty[b], kEpiWarps * C::CTAS);
     }
     mbar_init(&mma_done, 1);
     fence_mbar_init();
   }
   if (warp == 1) {
-    tmem_alloc(&tmem_slot, kTmemCols);
-    tmem_relinquish();
+    if (PAIR) {
+      tmem_alloc_pair(&tmem_slot, C::TMEM_COLS);
+      tmem_relinquish_pair();
+    } else {
+      tmem_alloc(&tmem_slot, C::TMEM_COLS);
+      tmem_relinquish();
+    }
   }
   if (warp == 2) {  // running sums of the groups' rows and activation tiles
     int rows_run = 0, tiles_run = 0;
@@ -119,7 +218,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (bad && blockIdx.x == 0) atomicCAS(p.err, 0, kMx4ErrCounts);
       // counts beyond the rows there are: the groups end with the rows
       const int first = (int)min(r - c, (long long)p.m), last = (int)min(r, (long long)p.m);
-      int t = (last - first + kTileN - 1) / kTileN;
+      int t = (last - first + C::NMAX - 1) / C::NMAX;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
         const int u = __shfl_up_sync(0xFFFFFFFFu, t, o);
@@ -136,9 +235,15 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
   tc_fence_before();
   __syncthreads();
+  if (PAIR) cluster_sync();
   tc_fence_after();
   const uint32_t tmem = tmem_slot;
   const long long total = (long long)tile0_[p.groups] * p.n_tiles;
+  // tiles of this CTA (pair, cluster): item0, item0 + step, ...; stages [k_lo, k_hi) of each
+  const long long item0 = blockIdx.x / n_ranks;
+  const long long step = SPLIT ? total + 1 : gridDim.x / n_ranks;  // a split's cluster has one tile
+  const int k_lo = SPLIT ? (int)((long long)p.k_steps * rank / n_ranks) : 0;
+  const int k_hi = SPLIT ? (int)((long long)p.k_steps * (rank + 1) / n_ranks) : p.k_steps;
 
   auto tile_at = [&](long long item) {
     const int xt = (int)(item / p.n_tiles);
@@ -149,158 +254,220 @@ __global__ void __launch_bounds__(kThreads, 1)
       else hi = mid;
     }
     const int first = row0_[lo], rows = row0_[lo + 1] - first, nt = tile0_[lo + 1] - tile0_[lo];
-    const int step = ((rows + nt - 1) / nt + 15) & ~15;  // equal tiles, a multiple of 16 rows
+    const int per = round_cols<C>((rows + nt - 1) / nt);  // equal tiles
     Tile t;
     t.g = lo;
-    t.f0 = (int)(item - (long long)xt * p.n_tiles) * kTileW;
-    const int i0 = (xt - tile0_[lo]) * step;
+    t.f0 = (int)(item - (long long)xt * p.n_tiles) * (kTileW * C::CTAS) + (PAIR ? (int)rank * kTileW : 0);
+    const int i0 = (xt - tile0_[lo]) * per;
     t.row0 = first + i0;
-    t.rows = max(0, min(step, rows - i0));
-    t.cols = max(16, (t.rows + 15) & ~15);
+    t.rows = min(per, rows - i0);
+    t.cols = round_cols<C>(t.rows);
     return t;
   };
+  auto start = [&] {
+    Cursor c;
+    c.item = item0;
+    c.ks = k_lo;
+    if (item0 < total) c.t = tile_at(item0);
+    return c;
+  };
+  auto advance = [&](Cursor &c, int by) {
+    c.ks += by;
+    while (c.ks >= k_hi && c.item < total) {
+      c.ks -= k_hi - k_lo;
+      c.item += step;
+      if (c.item < total) c.t = tile_at(c.item);
+    }
+  };
+  auto rank0 = [&](uint64_t *bar) { return PAIR ? mapa_shared(smem_addr(bar), 0) : smem_addr(bar); };
 
   if (warp == 0) {
     // ------------------------------------------------------------ codes
-    if (lane == 0) {
+    if (elect_one()) {
       prefetch_tmap(&tm_x);
       prefetch_tmap(&tm_w);
-      int s = 0, round = 0;
-      int last_round[kStages];
-#pragma unroll
-      for (int i = 0; i < kStages; ++i) last_round[i] = -1;
-      bool ok = true;
-      for (long long item = blockIdx.x; ok && item < total; item += gridDim.x) {
-        const Tile t = tile_at(item);
-        const int boxes = (t.cols + kBoxN - 1) / kBoxN;
-        for (int ks = 0; ks < p.k_steps; ++ks) {
-          if (round > 0 && !(ok = mbar_wait(&empty_[s], (round - 1) & 1, p.err, kMx4ErrWait))) break;
-          uint8_t *st = stages + s * kStageBytes;
-          mbar_arrive_expect_tx(&full_[s], (uint32_t)(kWBytes + boxes * kBoxN * 128));
-          tma_load_3d(st, &tm_w, &full_[s], ks * 128, t.f0, t.g);
-          for (int b = 0; b < boxes; ++b)
-            tma_load_2d(st + kWBytes + b * kBoxN * 128, &tm_x, &full_[s], ks * 128, t.row0 + b * kBoxN);
-          last_round[s] = round;
-          if (++s == kStages) {
-            s = 0;
-            ++round;
+    }
+    __syncwarp();
+    int s = 0, round = 0;
+    bool ok = true;
+    for (long long item = item0; ok && item < total; item += step) {
+      const Tile t = tile_at(item);
+      const int half = t.cols / C::CTAS, boxes = (half + p.box - 1) / p.box;
+      const int x0 = t.row0 + (PAIR ? (int)rank * half : 0);
+      const uint32_t tx = (uint32_t)(C::CTAS * (kWBytes + boxes * p.box * 128));
+      for (int ks = k_lo; ks < k_hi; ++ks) {
+        if (round > 0 && !(ok = mbar_wait(&empty_[s], (round - 1) & 1, p.err, kMx4ErrWait))) break;
+        if (elect_one()) {
+          if (PAIR && rank == 0 && round > 0) mbar_arrive_cluster(mapa_shared(smem_addr(&empty_[s]), 1));
+          uint8_t *st = stages + s * C::BYTES;
+          if (rank == 0 || SPLIT) mbar_arrive_expect_tx(&full_[s], tx);
+          if (PAIR) {
+            const uint32_t bar = mapa_shared(smem_addr(&full_[s]), 0);
+            tma_load_3d_pair(st, &tm_w, bar, ks * 128, t.f0, t.g);
+            for (int b = 0; b < boxes; ++b)
+              tma_load_2d_pair(st + kWBytes + b * p.box * 128, &tm_x, bar, ks * 128, x0 + b * p.box);
+          } else {
+            tma_load_3d(st, &tm_w, &full_[s], ks * 128, t.f0, t.g);
+            for (int b = 0; b < boxes; ++b)
+              tma_load_2d(st + kWBytes + b * p.box * 128, &tm_x, &full_[s], ks * 128, x0 + b * p.box);
           }
         }
+        __syncwarp();
+        if (++s == STAGES) {
+          s = 0;
+          ++round;
+        }
       }
-      if (!ok)  // copies in flight land before the CTA ends
-        for (int i = 0; i < kStages; ++i)
-          if (last_round[i] >= 0) mbar_wait(&full_[i], last_round[i] & 1, p.err, kMx4ErrWait);
+    }
+    if (!ok && (rank == 0 || SPLIT)) {
+      // copies in flight land before the CTA (pair) ends: stages below s have been loaded in this round
+      for (int i = 0; i < STAGES; ++i) {
+        const int last = i < s ? round : round - 1;
+        if (last >= 0) mbar_wait(&full_[i], last & 1, p.err, kMx4ErrWait);
+      }
     }
   } else if (warp == 1) {
-    // ------------------------------------------------------------ MMA
-    if (lane == 0) {
+    // ------------------------------------------------------------ MMA (rank 0 of a pair)
+    if (rank == 0 || SPLIT) {
       int s = 0, phase = 0, j = 0;
       bool ok = true;
-      const uint32_t sfw = tmem + kSfwCol, sfx = tmem + kSfxCol;
-      for (long long item = blockIdx.x; ok && item < total; item += gridDim.x, ++j) {
+      const uint32_t sfw = tmem + C::SFW_COL, sfx = tmem + C::SFX_COL;
+      for (long long item = item0; ok && item < total; item += step, ++j) {
         const Tile t = tile_at(item);
         const int buf = j & 1, rr = j >> 1;
         if (rr > 0 && !(ok = mbar_wait(&acc_empty[buf], (rr - 1) & 1, p.err, kMx4ErrWait))) break;
         tc_fence_after();
-        const uint32_t d = tmem + (uint32_t)(buf * kTileN);
-        const uint32_t id0 = idesc_mxf4(kTileW, t.cols, 0), id2 = idesc_mxf4(kTileW, t.cols, 2);
-        for (int ks = 0; ks < p.k_steps; ++ks) {
-          if (!(ok = mbar_wait(&full_[s], phase, p.err, kMx4ErrWait) && mbar_wait(&scaled_[s], phase, p.err, kMx4ErrWait))) break;
+        const uint32_t d = tmem + (uint32_t)(buf * C::NMAX);
+        const uint32_t id0 = idesc_mxf4(kTileW * C::CTAS, t.cols, 0), id2 = idesc_mxf4(kTileW * C::CTAS, t.cols, 2);
+        for (int ks = k_lo; ks < k_hi; ++ks) {
+          ok = PAIR ? mbar_wait_acquire_cluster(&scaled_[s], phase, p.err, kMx4ErrWait)
+                    : mbar_wait(&scaled_[s], phase, p.err, kMx4ErrWait);
+          if (!(ok = ok && mbar_wait(&full_[s], phase, p.err, kMx4ErrWait))) break;
           tc_fence_after();
-          const uint32_t st = smem_addr(stages + s * kStageBytes), sf = st + kWBytes + kXBytes;
-          const int mmas = min(4, (p.k - ks * kStageK + 63) / 64);
+          if (elect_one()) {
+            const uint32_t st = smem_addr(stages + s * C::BYTES), sf = st + kWBytes + C::X_BYTES;
+            const int mmas = (p.k - ks * kStageK + 63) / 64;  // 4, but for the end of K
 #pragma unroll
-          for (int w = 0; w < 2; ++w) {
-            utccp_atom(sfw + 4 * w, sf + w * kAtomBytes);
-            utccp_atom(sfx + 8 * w, sf + kSfw + 2 * w * kAtomBytes);
-            if (t.cols > 128) utccp_atom(sfx + 8 * w + 4, sf + kSfw + (2 * w + 1) * kAtomBytes);
+            for (int w = 0; w < 2; ++w) {
+              auto cp = [](uint32_t col, uint32_t atom) {
+                if (PAIR) utccp_atom_pair(col, atom);
+                else utccp_atom(col, atom);
+              };
+              cp(sfw + 4 * w, sf + w * kAtomBytes);
+              cp(sfx + 4 * C::X_GROUPS * w, sf + C::SFW + C::X_GROUPS * w * kAtomBytes);
+              if (C::X_GROUPS > 1) cp(sfx + 4 * C::X_GROUPS * w + 4, sf + C::SFW + (C::X_GROUPS * w + 1) * kAtomBytes);
+            }
+            const uint64_t wd = desc_sw128_kmajor(st), xd = desc_sw128_kmajor(st + kWBytes);
+#pragma unroll
+            for (int kk = 0; kk < 4; ++kk) {
+              if (kk < mmas) {
+                const uint32_t half = (uint32_t)(kk & 1) << 31;  // scale columns 2 and 3 of the word
+                const uint32_t fw = (sfw + 4 * (kk >> 1)) | half, fx = (sfx + 4 * C::X_GROUPS * (kk >> 1)) | half;
+                const uint32_t add = ks > k_lo || kk > 0;
+                if (PAIR) umma_mxf4_pair(d, wd + 2 * kk, xd + 2 * kk, kk & 1 ? id2 : id0, fw, fx, add);
+                else umma_mxf4(d, wd + 2 * kk, xd + 2 * kk, kk & 1 ? id2 : id0, fw, fx, add);
+              }
+            }
+            if (PAIR) umma_commit_pair(smem_addr(&empty_[s]));
+            else umma_commit(&empty_[s]);
+            if (ks + 1 == k_hi) {
+              if (PAIR) umma_commit_pair(smem_addr(&acc_full[buf]));
+              else umma_commit(&acc_full[buf]);
+            }
           }
-          const uint64_t wd = desc_sw128_kmajor(st), xd = desc_sw128_kmajor(st + kWBytes);
-          for (int kk = 0; kk < mmas; ++kk) {
-            const uint32_t half = (uint32_t)(kk & 1) << 31;  // scale columns 2 and 3 of the word
-            umma_mxf4(d, wd + 2 * kk, xd + 2 * kk, kk & 1 ? id2 : id0, (sfw + 4 * (kk >> 1)) | half,
-                      (sfx + 8 * (kk >> 1)) | half, (ks | kk) != 0);
-          }
-          umma_commit(&empty_[s]);
-          if (++s == kStages) {
+          __syncwarp();
+          if (++s == STAGES) {
             s = 0;
             phase ^= 1;
           }
         }
-        if (ok) umma_commit(&acc_full[buf]);
       }
-      umma_commit(&mma_done);  // no MMA is left when the tensor memory goes
+      // no MMA is left when the tensor memory goes
+      if (elect_one()) {
+        if (PAIR) umma_commit_pair(smem_addr(&mma_done));
+        else umma_commit(&mma_done);
+      }
+      __syncwarp();
       mbar_wait(&mma_done, 0, p.err, kMx4ErrWait);
     }
-  } else if (warp == 2) {
+  } else if (warp < 4 || warp >= 8) {
     // ------------------------------------------------------------ scales
-    // kAhead stages' copies are in flight; a stage is handed over when its own have landed
-    constexpr int kAhead = kStages - 2;  // so one stage is handed over while the oldest is still being read
-    long long issued = 0;
-    int s = 0, round = 0, done_s = 0;
-    bool ok = true;
-    auto hand_over = [&] {
-      fence_proxy_async_smem();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&scaled_[done_s]);
-      if (++done_s == kStages) done_s = 0;
-    };
-    for (long long item = blockIdx.x; ok && item < total; item += gridDim.x) {
-      const Tile t = tile_at(item);
-      const uint32_t *wsf = p.b_scales + (size_t)t.g * p.words * p.n;
-      for (int ks = 0; ks < p.k_steps; ++ks) {
-        if (round > 0 && !(ok = mbar_wait(&empty_[s], (round - 1) & 1, p.err, kMx4ErrWait))) break;
-        const uint32_t sf = smem_addr(stages + s * kStageBytes + kWBytes + kXBytes) + 16 * lane;
+    // one of two warps for the weights' words (sides 0) or the activations', every other stage each
+    const bool x_side = warp & 1;
+    const int first = warp >= 8 ? 1 : 0;
+    constexpr int XQ = (C::NMAX + 31) / 32;  // 32-row pieces of the activation rows
+    auto feed = [&](auto xs_) {
+      constexpr bool X = decltype(xs_)::value;
+      constexpr int Q = X ? XQ : 4;
+      uint32_t v[2][Q];
+      Cursor c = start();
+      advance(c, first);
+      auto fetch = [&](const Cursor &at) {
+        const int rows = X ? p.m : p.n, r0 = X ? at.t.row0 : at.t.f0;
+        const uint32_t *src = (X ? p.a_scales : p.b_scales + (size_t)at.t.g * p.words * p.n) + r0 + lane;
 #pragma unroll
         for (int w = 0; w < 2; ++w) {
-          const int kw = 2 * ks + w;
-          const bool in_k = kw < p.words;
-          const uint32_t *ws = wsf + (size_t)(in_k ? kw : 0) * p.n, *xs = p.a_scales + (size_t)(in_k ? kw : 0) * p.m;
+          const int kw = 2 * at.ks + w;
+          const uint32_t *row = src + (size_t)kw * rows;
 #pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            const int f = t.f0 + 32 * q + lane;
-            const bool in = in_k && f < p.n;
-            cp_async_4_zfill(sf + w * kAtomBytes + 4 * q, ws + (in ? f : 0), in);
-          }
-#pragma unroll
-          for (int q = 0; q < 8; ++q) {
-            if (32 * q >= t.cols) break;
-            const int r = t.row0 + 32 * q + lane;
-            const bool in = in_k && r < p.m;
-            cp_async_4_zfill(sf + kSfw + (2 * w + (q >> 2)) * kAtomBytes + 4 * (q & 3), xs + (in ? r : 0), in);
-          }
+          for (int q = 0; q < Q; ++q)
+            v[w][q] = kw < p.words && r0 + 32 * q + lane < rows && (!X || 32 * q < at.t.cols) ? __ldg(row + 32 * q) : 0u;
         }
-        cp_async_commit();
-        if (++s == kStages) {
-          s = 0;
+      };
+      if (c.item < total) fetch(c);
+      int s = first, round = 0;
+      while (c.item < total) {
+        if (round > 0 && !mbar_wait(&empty_[s], (round - 1) & 1, p.err, kMx4ErrWait)) break;
+        uint4 *sf = reinterpret_cast<uint4 *>(stages + s * C::BYTES + kWBytes + C::X_BYTES + (X ? C::SFW : 0)) + lane;
+#pragma unroll
+        for (int w = 0; w < 2; ++w)
+#pragma unroll
+          for (int q = 0; q < Q; q += 4)
+            sf[(X ? C::X_GROUPS * w + q / 4 : w) * (kAtomBytes / 16)] =
+                make_uint4(v[w][q], q + 1 < Q ? v[w][q + 1 < Q ? q + 1 : q] : 0u, q + 2 < Q ? v[w][q + 2 < Q ? q + 2 : q] : 0u,
+                           q + 3 < Q ? v[w][q + 3 < Q ? q + 3 : q] : 0u);
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) {
+          if (PAIR) mbar_arrive_release_cluster(rank0(&scaled_[s]));
+          else mbar_arrive(&scaled_[s]);
+        }
+        advance(c, 2);
+        if (c.item < total) fetch(c);
+        if ((s += 2) >= STAGES) {
+          s -= STAGES;
           ++round;
         }
-        if (++issued > kAhead) {
-          cp_async_wait<kAhead>();
-          hand_over();
-        }
       }
-    }
-    cp_async_wait<0>();
-    for (long long i = issued > kAhead ? issued - kAhead : 0; i < issued; ++i) hand_over();
-  } else if (warp >= 4) {
+    };
+    static_assert(STAGES % 2 == 0, "a warp's stages keep their parity around the ring");
+    if (x_side) feed(std::true_type{});
+    else feed(std::false_type{});
+  } else {
     // ------------------------------------------------------------ epilogue
     const int q = warp & 3;  // TMEM lane quarter
     int j = 0;
-    for (long long item = blockIdx.x; item < total; item += gridDim.x, ++j) {
+    for (long long item = item0; item < total; item += step, ++j) {
       const Tile t = tile_at(item);
       const int buf = j & 1;
       if (!mbar_wait(&acc_full[buf], (j >> 1) & 1, p.err, kMx4ErrWait)) break;
+      if (PAIR && rank == 0 && q == 0 && lane == 0) mbar_arrive_cluster(mapa_shared(smem_addr(&acc_full[buf]), 1));
       tc_fence_after();
       const int f = t.f0 + q * 32 + lane;
       const bool in = f < p.n;
-      const float bias = p.bias && in ? bf16_to_f32(__ldg(p.bias + (size_t)t.g * p.n + f)) : 0.f;
-      const uint32_t base = tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)(buf * kTileN);
+      const float bias = p.bias && in && !SPLIT ? bf16_to_f32(__ldg(p.bias + (size_t)t.g * p.n + f)) : 0.f;
+      const uint32_t base = tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)(buf * C::NMAX);
       for (int c0 = 0; c0 < t.rows; c0 += 32) {
         uint32_t v[32];
         tmem_ld_32_async(base + (uint32_t)c0, v);
         tmem_wait_ld(v);
-        if (!p.out_bf16) {
+        if (SPLIT) {
+          // this part of K: [column][feature], where the stages were (all of them have been read)
+          float *part = reinterpret_cast<float *>(stages) + c0 * kTileW + q * 32 + lane;
+#pragma unroll
+          for (int i = 0; i < 32; ++i)
+            if (c0 + i < t.rows) part[i * kTileW] = __uint_as_float(v[i]);
+        } else if (!p.out_bf16) {
           float *o = static_cast<float *>(p.out) + (size_t)(t.row0 + c0) * p.ldo + f;
 #pragma unroll
           for (int i = 0; i < 32; ++i)
@@ -314,9 +481,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           for (int i = 0; i < 32; i += 2) {
             const float v0 = __uint_as_float(v[i]) + bias, v1 = __uint_as_float(v[i + 1]) + bias;
             const float other = __shfl_xor_sync(0xFFFFFFFFu, odd ? v0 : v1, 1);
-            const float lo = odd ? other : v0, hi = odd ? v1 : other;
-            uint32_t both;
-            asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(both) : "f"(hi), "f"(lo));
+            const uint32_t both = pack_bf16x2(odd ? other : v0, odd ? v1 : other);
             if (c0 + i + odd >= t.rows) continue;
             uint16_t *dst = o + (size_t)i * p.ldo;
             if (fe + 1 < p.n && p.pair_stores) {
@@ -330,14 +495,46 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&acc_empty[buf]);
+      if (lane == 0) {
+        if (PAIR) mbar_arrive_cluster(rank0(&acc_empty[buf]));
+        else mbar_arrive(&acc_empty[buf]);
+      }
     }
   }
 
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  if (warp == 1) tmem_dealloc(tmem, kTmemCols);
+  if (SPLIT) {
+    // out = the parts of all ranks, added in rank order; rank r takes columns r, r + ranks, ...
+    cluster_sync();
+    if (item0 < total) {
+      const Tile t = tile_at(item0);
+      const int fl = threadIdx.x & (kTileW - 1), f = t.f0 + fl;
+      if (threadIdx.x < 2 * kTileW && f < p.n) {
+        const float bias = p.bias ? bf16_to_f32(__ldg(p.bias + (size_t)t.g * p.n + f)) : 0.f;
+        for (int c = (int)rank + (int)(threadIdx.x / kTileW) * (int)n_ranks; c < t.rows; c += 2 * (int)n_ranks) {
+          const uint32_t part = smem_addr(stages) + (uint32_t)(c * kTileW + fl) * 4;
+          float sum = 0.f;
+          for (uint32_t r = 0; r < n_ranks; ++r) sum += ld_cluster_f32(mapa_shared(part, r));
+          sum += bias;
+          const size_t o = (size_t)(t.row0 + c) * p.ldo + f;
+          if (p.out_bf16) static_cast<uint16_t *>(p.out)[o] = (uint16_t)pack_bf16x2(sum, 0.f);
+          else static_cast<float *>(p.out)[o] = sum;
+        }
+      }
+    }
+    __syncthreads();
+    cluster_sync();  // no CTA leaves while another may still read its part
+  }
+  if (PAIR) {
+    cluster_sync();
+    tc_fence_after();
+  }
+  if (warp == 1) {
+    if (PAIR) tmem_dealloc_pair(tmem, C::TMEM_COLS);
+    else tmem_dealloc(tmem, C::TMEM_COLS);
+  }
 }
 
 typedef CUresult (*EncodeFn)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *,
@@ -367,14 +564,55 @@ cudaError_t code_map(CUtensorMap *map, const void *base, int rank, int k, int ro
   return r == CUDA_SUCCESS ? cudaSuccess : cudaErrorInvalidValue;
 }
 
+
+
+template <class C>
+cudaError_t launch_cfg(const Mx4GemmArgs &a, Params &p, int n_sms, int ranks, cudaStream_t stream) {
+  constexpr int kTile = kTileW * C::CTAS;
+  p.n_tiles = (a.n + kTile - 1) / kTile;
+  // no more activation tiles than this, whatever the counts are
+  const long long x_tiles = a.counts ? (long long)a.m / C::NMAX + std::min(a.groups, a.m) : ((long long)a.m + C::NMAX - 1) / C::NMAX;
+  // one box where all tiles are alike; else two at most (16-row steps would be seven copies a stage)
+  if (a.counts) p.box = C::NMAX / C::CTAS / 2;
+  else p.box = round_cols<C>((a.m + (int)x_tiles - 1) / (int)x_tiles) / C::CTAS;
+  CUtensorMap tm_x, tm_w;
+  cudaError_t st;
+  if ((st = code_map(&tm_x, a.a, 2, a.k, a.m, 1, p.box))) return st;
+  if ((st = code_map(&tm_w, a.b, 3, a.k, a.n, a.groups, kTileW))) return st;
+  const long long tiles = x_tiles * p.n_tiles;
+  auto kern = mx4_gemm_kernel<C>;
+  if ((st = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM))) return st;
+  cudaLaunchConfig_t cfg{};
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = (unsigned)(C::SPLIT ? ranks : C::CTAS);
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = C::SMEM;
+  cfg.stream = stream;
+  cfg.attrs = attr;
+  cfg.numAttrs = C::SPLIT || C::PAIR ? 1 : 0;
+  long long at_once = n_sms;  // tiles in work side by side; the GPU's clusters may not hold every SM
+  if (C::PAIR) {
+    static const int pairs = [&] {
+      int n = 0;
+      cfg.gridDim = dim3((unsigned)(n_sms / 2 * 2));
+      return cudaOccupancyMaxActiveClusters(&n, kern, &cfg) == cudaSuccess && n > 0 ? n : 1;
+    }();
+    at_once = std::min(pairs, n_sms / 2);
+  }
+  cfg.gridDim = dim3((unsigned)(C::SPLIT ? tiles * ranks : C::CTAS * std::min(at_once, tiles)));
+  return cudaLaunchKernelEx(&cfg, kern, tm_x, tm_w, p);
+}
+
+using Pair = Cfg<true, 224, 6, false>;
+using Few = Cfg<false, 64, 8, false>;
+using FewSplit = Cfg<false, 64, 8, true>;
+
 }  // namespace
 
 cudaError_t launch_mx4_gemm(const Mx4GemmArgs &a, int n_sms, cudaStream_t stream) {
-  if (a.m == 0 || a.n == 0) return cudaSuccess;
-  CUtensorMap tm_x, tm_w;
-  cudaError_t st;
-  if ((st = code_map(&tm_x, a.a, 2, a.k, a.m, 1, kBoxN))) return st;
-  if ((st = code_map(&tm_w, a.b, 3, a.k, a.n, a.groups, kTileW))) return st;
+  if (a.m == 0 || a.n == 0 || a.groups == 0) return cudaSuccess;
   Params p{};
   p.m = a.m;
   p.n = a.n;
@@ -386,19 +624,17 @@ cudaError_t launch_mx4_gemm(const Mx4GemmArgs &a, int n_sms, cudaStream_t stream
   p.bias = a.bias;
   p.out = a.out;
   p.ldo = a.ldo;
-  p.n_tiles = (a.n + kTileW - 1) / kTileW;
   p.k_steps = (a.k + kStageK - 1) / kStageK;
   p.words = (a.k + 127) / 128;
   p.out_bf16 = a.out_bf16;
   p.pair_stores = a.ldo % 2 == 0 && (uintptr_t)a.out % 4 == 0;
   p.err = a.err;
-  // no more activation tiles than this, whatever the counts are
-  const long long x_tiles = a.counts ? (long long)a.m / kTileN + std::min(a.groups, a.m) : ((long long)a.m + kTileN - 1) / kTileN;
-  const unsigned grid = (unsigned)std::min<long long>(n_sms, x_tiles * p.n_tiles);
-  constexpr int smem = kStages * kStageBytes + 1024;
-  if ((st = cudaFuncSetAttribute(mx4_gemm_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem))) return st;
-  mx4_gemm_kernel<<<grid, kThreads, smem, stream>>>(tm_x, tm_w, p);
-  return cudaGetLastError();
+  if ((long long)a.m > 64ll * a.groups) return launch_cfg<Pair>(a, p, n_sms, 1, stream);
+  const long long tiles = ((long long)a.n + kTileW - 1) / kTileW * std::min(a.groups, a.m);
+  int ranks = 1;  // CTAs per tile: a power of two that leaves each at least two stages
+  while (ranks < 8 && 2 * ranks * tiles <= n_sms && 4 * ranks <= p.k_steps) ranks *= 2;
+  if (ranks > 1) return launch_cfg<FewSplit>(a, p, n_sms, ranks, stream);
+  return launch_cfg<Few>(a, p, n_sms, 1, stream);
 }
 
 }  // namespace oxg

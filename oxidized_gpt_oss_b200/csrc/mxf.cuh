@@ -90,6 +90,16 @@ __device__ __forceinline__ void utccp_atom(uint32_t taddr, uint32_t atom_saddr) 
   asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(d) : "memory");
 }
 
+// The same in both CTAs of a pair, each from its own shared memory.
+__device__ __forceinline__ void utccp_atom_pair(uint32_t taddr, uint32_t atom_saddr) {
+  uint64_t d = 0;
+  d |= (uint64_t)((atom_saddr >> 4) & 0x3FFFu);
+  d |= (uint64_t)1 << 16;
+  d |= (uint64_t)(128 >> 4) << 32;
+  d |= (uint64_t)1 << 46;
+  asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(d) : "memory");
+}
+
 // 1-D bulk copy global -> shared, completion counted on an mbarrier. Both
 // addresses 16-byte aligned, bytes a multiple of 16.
 __device__ __forceinline__ void bulk_load(void *smem_dst, const void *gsrc, uint32_t bytes, uint64_t *bar) {
