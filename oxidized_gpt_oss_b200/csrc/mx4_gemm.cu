@@ -21,9 +21,9 @@
 // memory in rank order (so a result does not depend on timing).
 //
 // CTAs walk their tiles with the weight tile fastest: CTAs side by side share activation rows, and a group's
-// weights stay in L2. Warps: 0 TMA (codes, 128-byte swizzle), 1 MMA, 2-3 and 8-9 scales (weights and
-// activations, each stage's by one of two warps, which fetches its next stage's words before it waits for
-// that stage's memory), 4-7 epilogue (two accumulators: one tile drains while the next is computed).
+// weights stay in L2. Warps: 0 TMA (codes, 128-byte swizzle), 1 MMA, 2-3 and 8-13 scales (four for the weights'
+// words and four for the activations', a stage each in turn; the words of a warp's next stage are on their way
+// while it waits for that stage's memory), 4-7 epilogue (two accumulators: one tile drains while the next is computed).
 // Every wait is bounded; one that runs out sets the error word and the CTA winds down.
 #include <cuda.h>
 
@@ -42,8 +42,9 @@ using namespace mxf;
 
 constexpr int kTileW = 128;           // weight rows per CTA
 constexpr int kStageK = 256;          // elements of K per stage: 128 bytes of codes
-constexpr int kThreads = 320;
 constexpr int kEpiWarps = 4;
+constexpr int kScaleWarps = 4;         // for each operand; a stage belongs to one of them
+constexpr int kThreads = 32 * (2 + kEpiWarps + 2 * kScaleWarps);
 constexpr int kWBytes = kTileW * 128;  // a stage's weight codes
 
 // PAIR: two CTAs per tile. NMAX: most activation rows per tile. SPLIT: a cluster per tile, K split.
@@ -62,6 +63,7 @@ struct Cfg {
   static constexpr uint32_t TMEM_COLS = COLS_USED <= 128 ? 128 : (COLS_USED <= 256 ? 256 : 512);
   static_assert(COLS_USED <= 512 && X_BYTES % 1024 == 0, "tensor memory, swizzle atoms");
   static_assert(!(PAIR && SPLIT), "a pair does not split K");
+  static_assert(STAGES >= kScaleWarps, "a scale warp goes around the ring at most once a step");
   static_assert(!SPLIT || STAGES * BYTES >= NMAX * kTileW * 4, "the split's partial sums use the stages' memory");
 };
 
@@ -105,6 +107,14 @@ __device__ __forceinline__ void tma_load_3d_pair(void *smem_dst, const void *tma
       "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes"
       " [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(smem_addr(smem_dst)),
       "l"(tmap), "r"(bar_cl), "r"(c0), "r"(c1), "r"(c2)
+      : "memory");
+}
+// Arrives on the barrier at this offset in both CTAs of the pair once every MMA this thread issued before has
+// completed.
+__device__ __forceinline__ void umma_commit_both(uint64_t *bar) {
+  asm volatile(
+      "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(smem_addr(bar)),
+      "h"((uint16_t)3)
       : "memory");
 }
 __device__ __forceinline__ float ld_cluster_f32(uint32_t addr_cl) {
@@ -275,7 +285,6 @@ __global__ void __launch_bounds__(kThreads, 1)
       for (int ks = k_lo; ks < k_hi; ++ks) {
         if (round > 0 && !(ok = mbar_wait(&empty_[s], (round - 1) & 1, p.err, kMx4ErrWait))) break;
         if (elect_one()) {
-          if (PAIR && rank == 0 && round > 0) mbar_arrive_cluster(mapa_shared(smem_addr(&empty_[s]), 1));
           uint8_t *st = stages + s * C::BYTES;
           if (rank == 0 || SPLIT) mbar_arrive_expect_tx(&full_[s], tx);
           if (PAIR) {
@@ -343,10 +352,10 @@ __global__ void __launch_bounds__(kThreads, 1)
                 else umma_mxf4(d, wd + 2 * kk, xd + 2 * kk, kk & 1 ? id2 : id0, fw, fx, add);
               }
             }
-            if (PAIR) umma_commit_pair(smem_addr(&empty_[s]));
+            if (PAIR) umma_commit_both(&empty_[s]);
             else umma_commit(&empty_[s]);
             if (ks + 1 == k_hi) {
-              if (PAIR) umma_commit_pair(smem_addr(&acc_full[buf]));
+              if (PAIR) umma_commit_both(&acc_full[buf]);
               else umma_commit(&acc_full[buf]);
             }
           }
@@ -367,48 +376,46 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
   } else if (warp < 4 || warp >= 8) {
     // ------------------------------------------------------------ scales
-    // one of two warps for the weights' words (sides 0) or the activations', every other stage each
-    const bool x_side = warp & 1;
-    const int first = warp >= 8 ? 1 : 0;
+    // the weights' words or the activations', every kScaleWarps-th stage
+    const int sw = warp < 4 ? warp - 2 : warp - 6;  // 0 .. 2 kScaleWarps - 1
+    const bool x_side = sw & 1;
+    const int first = sw >> 1;
     constexpr int XQ = (C::NMAX + 31) / 32;  // 32-row pieces of the activation rows
     auto feed = [&](auto xs_) {
       constexpr bool X = decltype(xs_)::value;
       constexpr int Q = X ? XQ : 4;
-      uint32_t v[2][2][Q];  // the words of this warp's next two stages
+      uint32_t v[2][Q];  // the words of this warp's next stage
       Cursor c = start();
       advance(c, first);
-      auto fetch = [&](uint32_t (&w2)[2][Q]) {
+      auto fetch = [&] {
         if (c.item >= total) return;
         const int rows = X ? p.m : p.n, r0 = X ? c.t.row0 : c.t.f0;
-        const uint32_t *src = (X ? p.a_scales : p.b_scales + (size_t)c.t.g * p.words * p.n) + r0 + lane;
+        const int in = min(rows - r0, X ? c.t.cols : kTileW) - lane;  // this lane's rows 32 q < in
+        const uint32_t *src = (X ? p.a_scales : p.b_scales + (size_t)c.t.g * p.words * p.n) + r0 + lane + (size_t)(2 * c.ks) * rows;
 #pragma unroll
         for (int w = 0; w < 2; ++w) {
-          const int kw = 2 * c.ks + w;
-          const uint32_t *row = src + (size_t)kw * rows;
+          const int lim = 2 * c.ks + w < p.words ? in : 0;
 #pragma unroll
-          for (int q = 0; q < Q; ++q)
-            w2[w][q] = kw < p.words && r0 + 32 * q + lane < rows && (!X || 32 * q < c.t.cols) ? __ldg(row + 32 * q) : 0u;
+          for (int q = 0; q < Q; ++q) v[w][q] = 32 * q < lim ? __ldg(src + 32 * q) : 0u;
+          src += rows;
         }
-        advance(c, 2);
+        advance(c, kScaleWarps);
       };
-      long long left = 0;  // this warp's stages
-      if (item0 < total)
-        left = ((total - 1 - item0) / step + 1) * (k_hi - k_lo) - first;
-      left = (left + 1) / 2;
-      fetch(v[0]);
-      fetch(v[1]);
+      // this warp's stages
+      const long long mine = item0 < total ? ((total - 1 - item0) / step + 1) * (k_hi - k_lo) - first : 0;
+      const long long left = (mine + kScaleWarps - 1) / kScaleWarps;
+      fetch();
       int s = first, round = 0;
-      bool ok = true;
-      auto hand_over = [&](uint32_t (&w2)[2][Q]) {
-        if (round > 0 && !(ok = mbar_wait(&empty_[s], (round - 1) & 1, p.err, kMx4ErrWait))) return;
+      for (long long i = 0; i < left; ++i) {
+        if (round > 0 && !mbar_wait(&empty_[s], (round - 1) & 1, p.err, kMx4ErrWait)) break;
         uint4 *sf = reinterpret_cast<uint4 *>(stages + s * C::BYTES + kWBytes + C::X_BYTES + (X ? C::SFW : 0)) + lane;
 #pragma unroll
         for (int w = 0; w < 2; ++w)
 #pragma unroll
           for (int q = 0; q < Q; q += 4)
             sf[(X ? C::X_GROUPS * w + q / 4 : w) * (kAtomBytes / 16)] =
-                make_uint4(w2[w][q], q + 1 < Q ? w2[w][q + 1 < Q ? q + 1 : q] : 0u, q + 2 < Q ? w2[w][q + 2 < Q ? q + 2 : q] : 0u,
-                           q + 3 < Q ? w2[w][q + 3 < Q ? q + 3 : q] : 0u);
+                make_uint4(v[w][q], q + 1 < Q ? v[w][q + 1 < Q ? q + 1 : q] : 0u, q + 2 < Q ? v[w][q + 2 < Q ? q + 2 : q] : 0u,
+                           q + 3 < Q ? v[w][q + 3 < Q ? q + 3 : q] : 0u);
         // The tensor cores read this CTA's own shared memory, which the fence has made ready for them before
         // the barrier (rank 0's, in a pair) can move; a release at cluster scope would wait for the loads
         // above as well (104 against 79 us at 8192 x 5120 x 2880).
@@ -418,18 +425,13 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (PAIR) mbar_arrive_cluster(rank0(&scaled_[s]));
           else mbar_arrive(&scaled_[s]);
         }
-        fetch(w2);
-        if ((s += 2) >= STAGES) {
+        fetch();
+        if ((s += kScaleWarps) >= STAGES) {
           s -= STAGES;
           ++round;
         }
-      };
-      for (long long i = 0; ok && i < left; i += 2) {
-        hand_over(v[0]);
-        if (ok && i + 1 < left) hand_over(v[1]);
       }
     };
-    static_assert(STAGES % 2 == 0, "a warp's stages keep their parity around the ring");
     if (x_side) feed(std::true_type{});
     else feed(std::false_type{});
   } else {
@@ -440,7 +442,6 @@ __global__ void __launch_bounds__(kThreads, 1)
       const Tile t = tile_at(item);
       const int buf = j & 1;
       if (!mbar_wait(&acc_full[buf], (j >> 1) & 1, p.err, kMx4ErrWait)) break;
-      if (PAIR && rank == 0 && q == 0 && lane == 0) mbar_arrive_cluster(mapa_shared(smem_addr(&acc_full[buf]), 1));
       tc_fence_after();
       const int f = t.f0 + q * 32 + lane;
       const bool in = f < p.n;
