@@ -21,9 +21,9 @@
 // memory in rank order (so a result does not depend on timing).
 //
 // CTAs walk their tiles with the weight tile fastest: CTAs side by side share activation rows, and a group's
-// weights stay in L2. Warps: 0 TMA (codes, 128-byte swizzle), 1 MMA, 2-3 and 8-13 scales (four for the weights'
+// weights stay in L2. Warps: 0 TMA (codes, 128-byte swizzle), 1 MMA, 2-3 and 12-17 scales (four for the weights'
 // words and four for the activations', a stage each in turn; the words of a warp's next stage are on their way
-// while it waits for that stage's memory), 4-7 epilogue (two accumulators: one tile drains while the next is computed).
+// while it waits for that stage's memory), 4-11 epilogue (two accumulators: one tile drains while the next is computed).
 // Every wait is bounded; one that runs out sets the error word and the CTA winds down.
 #include <cuda.h>
 
@@ -42,7 +42,7 @@ using namespace mxf;
 
 constexpr int kTileW = 128;           // weight rows per CTA
 constexpr int kStageK = 256;          // elements of K per stage: 128 bytes of codes
-constexpr int kEpiWarps = 4;
+constexpr int kEpiWarps = 8;           // two for each quarter of the TMEM lanes, taking 32 columns in turn
 constexpr int kScaleWarps = 4;         // for each operand; a stage belongs to one of them
 constexpr int kThreads = 32 * (2 + kEpiWarps + 2 * kScaleWarps);
 constexpr int kWBytes = kTileW * 128;  // a stage's weight codes
@@ -144,8 +144,7 @@ __device__ __forceinline__ bool elect_one() {
 
 // A CTA's way through its tiles' stages.
 struct Cursor {
-  long long item;
-  int ks;
+  int item, ks;
   Tile t;
 };
 
@@ -225,15 +224,15 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (PAIR) cluster_sync();
   tc_fence_after();
   const uint32_t tmem = tmem_slot;
-  const long long total = (long long)tile0_[p.groups] * p.n_tiles;
+  const int total = tile0_[p.groups] * p.n_tiles;  // the launch has checked that this fits
   // tiles of this CTA (pair, cluster): item0, item0 + step, ...; stages [k_lo, k_hi) of each
-  const long long item0 = blockIdx.x / n_ranks;
-  const long long step = SPLIT ? total + 1 : gridDim.x / n_ranks;  // a split's cluster has one tile
+  const int item0 = (int)(blockIdx.x / n_ranks);
+  const int step = SPLIT ? total : (int)(gridDim.x / n_ranks);  // a split's cluster has one tile
   const int k_lo = SPLIT ? (int)((long long)p.k_steps * rank / n_ranks) : 0;
   const int k_hi = SPLIT ? (int)((long long)p.k_steps * (rank + 1) / n_ranks) : p.k_steps;
 
-  auto tile_at = [&](long long item) {
-    const int xt = (int)(item / p.n_tiles);
+  auto tile_at = [&](int item) {
+    const int xt = item / p.n_tiles;
     int lo = 0, hi = p.groups;  // the last group that starts at or before xt: empty ones before it start there too
     while (hi - lo > 1) {
       const int mid = (lo + hi) >> 1;
@@ -244,7 +243,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int per = round_cols<C>((rows + nt - 1) / nt);  // equal tiles
     Tile t;
     t.g = lo;
-    t.f0 = (int)(item - (long long)xt * p.n_tiles) * (kTileW * C::CTAS) + (PAIR ? (int)rank * kTileW : 0);
+    t.f0 = (item - xt * p.n_tiles) * (kTileW * C::CTAS) + (PAIR ? (int)rank * kTileW : 0);
     const int i0 = (xt - tile0_[lo]) * per;
     t.row0 = first + i0;
     t.rows = min(per, rows - i0);
@@ -277,7 +276,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     __syncwarp();
     int s = 0, round = 0;
     bool ok = true;
-    for (long long item = item0; ok && item < total; item += step) {
+    for (int item = item0; ok && item < total; item += step) {
       const Tile t = tile_at(item);
       const int half = t.cols / C::CTAS, boxes = (half + p.box - 1) / p.box;
       const int x0 = t.row0 + (PAIR ? (int)rank * half : 0);
@@ -318,13 +317,14 @@ __global__ void __launch_bounds__(kThreads, 1)
       int s = 0, phase = 0, j = 0;
       bool ok = true;
       const uint32_t sfw = tmem + C::SFW_COL, sfx = tmem + C::SFX_COL;
-      for (long long item = item0; ok && item < total; item += step, ++j) {
-        const Tile t = tile_at(item);
+      int next_cols = item0 < total ? tile_at(item0).cols : 0;
+      for (int item = item0; ok && item < total; item += step, ++j) {
+        const int cols = next_cols;
         const int buf = j & 1, rr = j >> 1;
         if (rr > 0 && !(ok = mbar_wait(&acc_empty[buf], (rr - 1) & 1, p.err, kMx4ErrWait))) break;
         tc_fence_after();
         const uint32_t d = tmem + (uint32_t)(buf * C::NMAX);
-        const uint32_t id0 = idesc_mxf4(kTileW * C::CTAS, t.cols, 0), id2 = idesc_mxf4(kTileW * C::CTAS, t.cols, 2);
+        const uint32_t id0 = idesc_mxf4(kTileW * C::CTAS, cols, 0), id2 = idesc_mxf4(kTileW * C::CTAS, cols, 2);
         for (int ks = k_lo; ks < k_hi; ++ks) {
           if (!(ok = mbar_wait(&scaled_[s], phase, p.err, kMx4ErrWait) && mbar_wait(&full_[s], phase, p.err, kMx4ErrWait))) break;
           tc_fence_after();
@@ -360,6 +360,8 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
           }
           __syncwarp();
+          // the next tile's width while the tensor cores have work in hand, not between the two tiles
+          if (ks == k_lo && item + step < total) next_cols = tile_at(item + step).cols;
           if (++s == STAGES) {
             s = 0;
             phase ^= 1;
@@ -374,10 +376,10 @@ __global__ void __launch_bounds__(kThreads, 1)
       __syncwarp();
       mbar_wait(&mma_done, 0, p.err, kMx4ErrWait);
     }
-  } else if (warp < 4 || warp >= 8) {
+  } else if (warp < 4 || warp >= 4 + kEpiWarps) {
     // ------------------------------------------------------------ scales
     // the weights' words or the activations', every kScaleWarps-th stage
-    const int sw = warp < 4 ? warp - 2 : warp - 6;  // 0 .. 2 kScaleWarps - 1
+    const int sw = warp < 4 ? warp - 2 : warp - 2 - kEpiWarps;  // 0 .. 2 kScaleWarps - 1
     const bool x_side = sw & 1;
     const int first = sw >> 1;
     constexpr int XQ = (C::NMAX + 31) / 32;  // 32-row pieces of the activation rows
@@ -402,11 +404,11 @@ __global__ void __launch_bounds__(kThreads, 1)
         advance(c, kScaleWarps);
       };
       // this warp's stages
-      const long long mine = item0 < total ? ((total - 1 - item0) / step + 1) * (k_hi - k_lo) - first : 0;
-      const long long left = (mine + kScaleWarps - 1) / kScaleWarps;
+      const int mine = item0 < total ? ((total - 1 - item0) / step + 1) * (k_hi - k_lo) - first : 0;
+      const int left = (mine + kScaleWarps - 1) / kScaleWarps;
       fetch();
       int s = first, round = 0;
-      for (long long i = 0; i < left; ++i) {
+      for (int i = 0; i < left; ++i) {
         if (round > 0 && !mbar_wait(&empty_[s], (round - 1) & 1, p.err, kMx4ErrWait)) break;
         uint4 *sf = reinterpret_cast<uint4 *>(stages + s * C::BYTES + kWBytes + C::X_BYTES + (X ? C::SFW : 0)) + lane;
 #pragma unroll
@@ -436,9 +438,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     else feed(std::false_type{});
   } else {
     // ------------------------------------------------------------ epilogue
-    const int q = warp & 3;  // TMEM lane quarter
+    const int q = warp & 3, half = (warp - 4) >> 2;  // TMEM lane quarter; which 32-column chunks
     int j = 0;
-    for (long long item = item0; item < total; item += step, ++j) {
+    for (int item = item0; item < total; item += step, ++j) {
       const Tile t = tile_at(item);
       const int buf = j & 1;
       if (!mbar_wait(&acc_full[buf], (j >> 1) & 1, p.err, kMx4ErrWait)) break;
@@ -448,7 +450,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const float bias = p.bias && in && !SPLIT ? bf16_to_f32(__ldg(p.bias + (size_t)t.g * p.n + f)) : 0.f;
       const uint32_t base = tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)(buf * C::NMAX);
       const bool whole = t.f0 + kTileW <= p.n && p.pair_stores;  // no feature of the tile is missing
-      for (int c0 = 0; c0 < t.rows; c0 += 32) {
+      for (int c0 = 32 * half; c0 < t.rows; c0 += 64) {
         uint32_t v[32];
         tmem_ld_32_async(base + (uint32_t)c0, v);
         tmem_wait_ld(v);
@@ -591,6 +593,7 @@ cudaError_t launch_cfg(const Mx4GemmArgs &a, Params &p, int n_sms, int ranks, cu
   if ((st = code_map(&tm_x, a.a, 2, a.k, a.m, 1, p.box))) return st;
   if ((st = code_map(&tm_w, a.b, 3, a.k, a.n, a.groups, kTileW))) return st;
   const long long tiles = x_tiles * p.n_tiles;
+  if (tiles > 0x3FFFFFFF || tiles * p.k_steps > 0x7FFFFFFF) return cudaErrorInvalidValue;  // no GPU's memory holds such operands
   auto kern = mx4_gemm_kernel<C>;
   if ((st = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM))) return st;
   cudaLaunchConfig_t cfg{};
