@@ -28,6 +28,7 @@
 #include <cuda.h>
 
 #include <algorithm>
+#include <atomic>
 #include <type_traits>
 
 #include "common.cuh"
@@ -595,7 +596,13 @@ cudaError_t launch_cfg(const Mx4GemmArgs &a, Params &p, int n_sms, int ranks, cu
   const long long tiles = x_tiles * p.n_tiles;
   if (tiles > 0x3FFFFFFF || tiles * p.k_steps > 0x7FFFFFFF) return cudaErrorInvalidValue;  // no GPU's memory holds such operands
   auto kern = mx4_gemm_kernel<C>;
-  if ((st = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM))) return st;
+  static std::atomic<uint64_t> ready{0};  // a bit for each device (of the first 64) that knows the attribute
+  int dev = 0;
+  if ((st = cudaGetDevice(&dev))) return st;
+  if (dev >= 64 || !(ready.load(std::memory_order_relaxed) >> dev & 1)) {
+    if ((st = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM))) return st;
+    if (dev < 64) ready.fetch_or(1ull << dev, std::memory_order_relaxed);
+  }
   cudaLaunchConfig_t cfg{};
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;

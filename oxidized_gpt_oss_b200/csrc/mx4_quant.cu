@@ -11,8 +11,8 @@
 //
 // Bound: HBM. A thread owns 8 consecutive elements (one 16-byte load of 16-bit types, two of f32) and a
 // block is four neighbouring lanes, which share the largest magnitude by two shuffles; the codes leave as
-// one 4-byte word per thread. Each thread issues the loads of kUnr chunks, a grid's width apart, before it
-// works on the first.
+// one 4-byte word per thread. Each thread issues 64 bytes of loads, chunks a grid's width apart, before it works
+// on the first.
 #include "common.cuh"
 #include "mx4.h"
 
@@ -105,17 +105,28 @@ __device__ __forceinline__ int scale_byte(uint32_t top, int rule) {
 }
 __device__ __forceinline__ float inverse_scale(int byte) { return __uint_as_float((uint32_t)(254 - byte) << 23); }
 
-// max over the four lanes of a block
-__device__ __forceinline__ uint32_t block_max(uint32_t v) {
-  v = max(v, __shfl_xor_sync(0xFFFFFFFFu, v, 1));
-  return max(v, __shfl_xor_sync(0xFFFFFFFFu, v, 2));
+// max and min that keep a NaN
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float min_nan(float a, float b) {
+  float r;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+// f32 bits of a block's largest magnitude (NaN if it holds one), shared by its four lanes
+__device__ __forceinline__ uint32_t block_top(const float (&v)[8]) {
+  float t = fabsf(v[0]);
+#pragma unroll
+  for (int i = 1; i < 8; ++i) t = max_nan(t, fabsf(v[i]));
+  t = max_nan(t, __shfl_xor_sync(0xFFFFFFFFu, t, 1));
+  return __float_as_uint(max_nan(t, __shfl_xor_sync(0xFFFFFFFFu, t, 2)));
 }
 
 __device__ __forceinline__ uint32_t quantize8(const float (&v)[8], int rule, int *byte) {
-  uint32_t top = 0u;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(v[i]) & 0x7FFFFFFFu);
-  top = block_max(top);
+  const uint32_t top = block_top(v);
   if (top >= 0x7F800000u) {
     *byte = 255;
     return 0u;
@@ -130,14 +141,16 @@ __device__ __forceinline__ double swiglu_f64(float gf, float uf, float alpha, fl
   return g * (1.0 / (1.0 + exp(-(double)alpha * g))) * (u + 1.0);
 }
 
-// Eight SwiGLU outputs from their gate / up pairs, quantised as the exact values would be. The f32 value is
-// within (|alpha g| + 9) 2^-24 of the exact one, relatively: one rounding of alpha g, which the exponential
-// turns into |alpha g| 2^-24; at most 2 ulp of expf; the roundings of the sum, the quotient, u + 1 and two
-// products. While -alpha g <= 80 that is below kTol = 2^-17. So where the block's largest magnitude or a
-// scaled element lies within kTol of a border between two scales or two codes (seen by rounding both
-// (1 - kTol) and (1 + kTol) times the value), where alpha g < -80, or where a product has left the
-// range in which f32 is that exact, the block's four lanes evaluate it again in f64: about 1 block in 300
-// of normally distributed inputs, so codes do not depend on which exponential computed them.
+// Eight SwiGLU outputs from their gate / up pairs, quantised as the exact values would be. The f32 value comes
+// from the hardware's exponential and reciprocal (ten instructions instead of forty: with expf and the IEEE
+// quotient the kernel took 210 us for 32768 x 2880 from bf16). For g >= 2^-40 or 0 and x = -alpha g <= 40 its
+// relative error stays below kTol = 2^-17 = 128 2^-24: log2 e, -alpha log2 e and its product with g are rounded,
+// 2.5 2^-24 |x| in e^x; ex2 adds 2^-22, the reciprocal 2^-23, the sum, u + 1 and two products 2^-24 each, 110
+// 2^-24 in all. No intermediate leaves f32's normal range (|u + 1| is 0 or at least 2^-24, the sigmoid at least
+// e^-40 / 2). So where the block's largest magnitude or a scaled element lies within kTol of a border between
+// two scales or two codes (seen by rounding both (1 - kTol) and (1 + kTol) times the value), or where a gate lies
+// outside that range, the block's four lanes evaluate it again in f64: about 1 block in 300 of normally
+// distributed inputs. The codes then do not depend on which exponential computed them.
 constexpr float kTol = 0x1p-17f;
 __device__ __forceinline__ uint32_t swiglu_quantize8_f64(const float (&gu)[16], float alpha, float limit, int rule, int *byte,
                                                       uint32_t lanes) {
@@ -145,12 +158,16 @@ __device__ __forceinline__ uint32_t swiglu_quantize8_f64(const float (&gu)[16], 
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     h[i] = swiglu_f64(gu[2 * i], gu[2 * i + 1], alpha, limit);
-    top = fabs(h[i]) > top ? fabs(h[i]) : top;
+    top = top != top || fabs(h[i]) <= top ? top : fabs(h[i]);  // a NaN stays
   }
 #pragma unroll
   for (int o = 1; o <= 2; o <<= 1) {
     const double other = __shfl_xor_sync(lanes, top, o);
-    top = other > top ? other : top;
+    top = top != top || other <= top ? top : other;
+  }
+  if (!(top < 0x1p128)) {  // what f32 does not hold
+    *byte = 255;
+    return 0u;
   }
   const long long bits = __double_as_longlong(top);
   int b = (int)(bits >> 52) - 1023 + 127 - 2;
@@ -166,21 +183,22 @@ __device__ __forceinline__ uint32_t swiglu_quantize8_f64(const float (&gu)[16], 
   return w;
 }
 __device__ __forceinline__ uint32_t swiglu_quantize8(const float (&gu)[16], float alpha, float limit, int rule, int *byte) {
+  const float c = -alpha * 1.4426950408889634f;  // e^(-alpha g) = 2^(c g)
   float h[8];
-  uint32_t top = 0u;
   bool close = false;
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    float g = gu[2 * i], u = gu[2 * i + 1];
-    g = g > limit ? limit : g;
-    u = u < -limit ? -limit : (u > limit ? limit : u);
-    const float x = -alpha * g, up = u + 1.0f;
-    h[i] = g * (1.0f / (1.0f + expf(x))) * up;
-    close |= x > 80.f || (fabsf(h[i]) < 0x1p-100f && g != 0.f && up != 0.f);
-    top = max(top, __float_as_uint(h[i]) & 0x7FFFFFFFu);
+    const float g = min_nan(gu[2 * i], limit), u = max_nan(min_nan(gu[2 * i + 1], limit), -limit);
+    const float x = c * g;
+    float e, r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(x));
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + e));
+    h[i] = g * r * (u + 1.0f);
+    close |= x > 57.f || (fabsf(g) < 0x1p-40f && g != 0.f);  // 40 log2 e
   }
-  top = block_max(top);
+  const uint32_t top = block_top(h);
   const bool finite = top < 0x7F800000u;
+  close |= top == 0x7F800000u;  // an overflow, perhaps only of the f32 arithmetic
   const float t = __uint_as_float(top);
   *byte = finite ? scale_byte(top, rule) : 255;
   const float inv = inverse_scale(finite ? *byte : 1);
@@ -188,36 +206,55 @@ __device__ __forceinline__ uint32_t swiglu_quantize8(const float (&gu)[16], floa
   close |= w != w1 || scale_byte(__float_as_uint(t * (1.0f - kTol)), rule) != scale_byte(__float_as_uint(t * (1.0f + kTol)), rule);
   const int lane = threadIdx.x & 31;
   const uint32_t lanes = 0xFu << (lane & ~3);
-  if (((__ballot_sync(0xFFFFFFFFu, close && finite) & lanes) != 0u))  // the four lanes of a block go together
+  if ((__ballot_sync(0xFFFFFFFFu, close) & lanes) != 0u)  // the four lanes of a block go together
     return swiglu_quantize8_f64(gu, alpha, limit, rule, byte, lanes);
   return finite ? w : 0u;
 }
 
-template <int T, bool SWIGLU, bool VEC, int UNR>
-__global__ void __launch_bounds__(kThreads) mx4_quantize_kernel(const Mx4QuantArgs a, size_t n_chunks) {
+// n / d for n below 2^32 by a multiplication (Granlund and Montgomery, "Division by invariant integers using
+// multiplication", 1994): the compiler's division costs as much as a chunk's arithmetic.
+struct Div {
+  uint32_t d, mul, shift;
+  explicit Div(uint32_t d_) : d(d_) {
+    uint32_t l = 0;
+    while (l < 32 && (1ull << l) < d) ++l;
+    mul = (uint32_t)((((1ull << l) - d) << 32) / d + 1);
+    shift = l ? l - 1 : 0;
+    if (d == 1) mul = 0;
+  }
+  __device__ __forceinline__ uint32_t quotient(uint32_t n) const {
+    if (d == 1) return n;
+    const uint32_t t = __umulhi(mul, n);
+    return (t + ((n - t) >> 1)) >> shift;
+  }
+};
+
+// How rows lie: one after another with scales in rows and no factors (a chunk's place is its number), on the
+// 16-byte grid with any pitch, or anyhow.
+enum Lay { kFlat, kGrid, kAny };
+
+template <int T, bool SWIGLU, Lay LAY, int UNR>
+__global__ void __launch_bounds__(kThreads) mx4_quantize_kernel(const Mx4QuantArgs a, size_t n_chunks, const Div per_row) {
   constexpr int N = SWIGLU ? 16 : 8;
-  const uint32_t per_row = (uint32_t)(a.cols / 8);
   const size_t stride = (size_t)gridDim.x * kThreads;
   // every lane of a warp makes the same rounds (shuffles below); chunks come in fours, so blocks stay whole
   for (size_t c0 = (size_t)blockIdx.x * kThreads + threadIdx.x; c0 - (threadIdx.x & 31) < n_chunks; c0 += UNR * stride) {
-    Raw<T, N, VEC> raw[UNR];
+    Raw<T, N, LAY != kAny> raw[UNR];
     size_t row[UNR];
     uint32_t col[UNR];
 #pragma unroll
     for (int u = 0; u < UNR; ++u) {
       const size_t c = c0 + u * stride;
-      if (n_chunks <= 0xFFFFFFFFull) {
-        row[u] = (uint32_t)c / per_row;
-        col[u] = (uint32_t)c - (uint32_t)row[u] * per_row;
-      } else {
-        row[u] = c / per_row;
-        col[u] = (uint32_t)(c - row[u] * per_row);
+      if (LAY != kFlat) {
+        row[u] = n_chunks <= 0xFFFFFFFFull ? per_row.quotient((uint32_t)c) : c / per_row.d;
+        col[u] = (uint32_t)(c - row[u] * per_row.d);
       }
+      const size_t at = LAY == kFlat ? c * N : row[u] * a.ld + (size_t)col[u] * N;
       if (c < n_chunks)
-        raw[u].load(static_cast<const uint8_t *>(a.x) + (row[u] * a.ld + (size_t)col[u] * N) * Elem<T>::kBytes);
+        raw[u].load(static_cast<const uint8_t *>(a.x) + at * Elem<T>::kBytes);
       else
 #pragma unroll
-        for (int i = 0; i < Raw<T, N, VEC>::kWords; ++i) raw[u].w[i] = make_uint4(0u, 0u, 0u, 0u);
+        for (int i = 0; i < Raw<T, N, LAY != kAny>::kWords; ++i) raw[u].w[i] = make_uint4(0u, 0u, 0u, 0u);
     }
 #pragma unroll
     for (int u = 0; u < UNR; ++u) {
@@ -229,7 +266,7 @@ __global__ void __launch_bounds__(kThreads) mx4_quantize_kernel(const Mx4QuantAr
       if constexpr (SWIGLU) {
         w = swiglu_quantize8(v, a.alpha, a.limit, a.rule, &byte);
       } else {
-        if (a.row_scale) {
+        if (LAY != kFlat && a.row_scale) {
           const float f = c < n_chunks ? __ldg(a.row_scale + row[u]) : 0.f;
 #pragma unroll
           for (int i = 0; i < N; ++i) v[i] = __fmul_rn(v[i], f);
@@ -239,13 +276,13 @@ __global__ void __launch_bounds__(kThreads) mx4_quantize_kernel(const Mx4QuantAr
       if (c >= n_chunks) continue;
       reinterpret_cast<uint32_t *>(a.blocks)[c] = w;
       if ((c & 3) == 0) {
-        if (!a.tiled) {
+        if (LAY == kFlat || !a.tiled) {
           a.scales[c >> 2] = (uint8_t)byte;
         } else {
           const uint32_t kb = col[u] >> 2;
           uint8_t *d = a.scales + ((size_t)(kb >> 2) * a.rows + row[u]) * 4;
           d[kb & 3] = (uint8_t)byte;
-          if (col[u] + 4 == per_row)  // zero where the row ends inside a 128-element stretch
+          if (col[u] + 4 == per_row.d)  // zero where the row ends inside a 128-element stretch
             for (uint32_t j = (kb & 3) + 1; j < 4; ++j) d[j] = 0;
         }
       }
@@ -269,19 +306,30 @@ __global__ void __launch_bounds__(kThreads)
   }
 }
 
-template <int T, bool SWIGLU, bool VEC>
-cudaError_t launch_quant(const Mx4QuantArgs &a, int n_sms, cudaStream_t stream) {
-  constexpr int UNR = 1;
-  const size_t n_chunks = a.rows * (a.cols / 8);
+template <int T, bool SWIGLU, Lay LAY, int UNR>
+cudaError_t launch_unr(const Mx4QuantArgs &a, size_t n_chunks, int n_sms, cudaStream_t stream) {
   const size_t want = (n_chunks + (size_t)kThreads * UNR - 1) / ((size_t)kThreads * UNR), cap = (size_t)n_sms * 8;
-  mx4_quantize_kernel<T, SWIGLU, VEC, UNR><<<(unsigned)(want < cap ? want : cap), kThreads, 0, stream>>>(a, n_chunks);
+  mx4_quantize_kernel<T, SWIGLU, LAY, UNR><<<(unsigned)(want < cap ? want : cap), kThreads, 0, stream>>>(
+      a, n_chunks, Div((uint32_t)(a.cols / 8)));
   return cudaGetLastError();
+}
+template <int T, bool SWIGLU, Lay LAY>
+cudaError_t launch_lay(const Mx4QuantArgs &a, int n_sms, cudaStream_t stream) {
+  const size_t n_chunks = a.rows * (a.cols / 8);
+  // chunks per thread in flight: 64 bytes of loads, once there is a chunk for every thread that fits the GPU
+  constexpr int UNR = 4 / (Elem<T>::kBytes / 2) / (SWIGLU ? 2 : 1);
+  if (n_chunks <= (size_t)n_sms * 2048) return launch_unr<T, SWIGLU, LAY, 1>(a, n_chunks, n_sms, stream);
+  return launch_unr<T, SWIGLU, LAY, UNR>(a, n_chunks, n_sms, stream);
+}
+template <int T, bool SWIGLU>
+cudaError_t launch_op(const Mx4QuantArgs &a, int n_sms, cudaStream_t stream) {
+  if ((uintptr_t)a.x % 16 != 0 || (a.rows > 1 && a.ld * Elem<T>::kBytes % 16 != 0)) return launch_lay<T, SWIGLU, kAny>(a, n_sms, stream);
+  const bool flat = (a.rows == 1 || a.ld == a.cols * (SWIGLU ? 2 : 1)) && !a.tiled && !a.row_scale;
+  return flat ? launch_lay<T, SWIGLU, kFlat>(a, n_sms, stream) : launch_lay<T, SWIGLU, kGrid>(a, n_sms, stream);
 }
 template <int T>
 cudaError_t launch_typed(const Mx4QuantArgs &a, bool swiglu, int n_sms, cudaStream_t stream) {
-  const bool vec = (uintptr_t)a.x % 16 == 0 && a.ld * Elem<T>::kBytes % 16 == 0;
-  if (swiglu) return vec ? launch_quant<T, true, true>(a, n_sms, stream) : launch_quant<T, true, false>(a, n_sms, stream);
-  return vec ? launch_quant<T, false, true>(a, n_sms, stream) : launch_quant<T, false, false>(a, n_sms, stream);
+  return swiglu ? launch_op<T, true>(a, n_sms, stream) : launch_op<T, false>(a, n_sms, stream);
 }
 
 }  // namespace

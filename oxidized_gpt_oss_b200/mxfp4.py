@@ -25,6 +25,15 @@ from . import abi
 _default_ctx = None
 
 
+def _bind(ctx: abi.Context) -> abi.Context:
+    """Puts the context on torch's current stream of its device."""
+    # the raw handle where this torch has it: the Stream object costs 3 us a call
+    raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+    stream = raw(ctx.device) if raw is not None else torch.cuda.current_stream(ctx.device).cuda_stream
+    abi.check(ctx.lib.oxg_ctx_set_stream(ctx.handle, stream), ctx.handle)
+    return ctx
+
+
 def context(ctx: abi.Context | None = None) -> abi.Context:
     """The given context, or a per-process default one on the current device,
     bound to torch's current stream."""
@@ -33,8 +42,7 @@ def context(ctx: abi.Context | None = None) -> abi.Context:
         if _default_ctx is None:
             _default_ctx = abi.Context(torch.cuda.current_device())
         ctx = _default_ctx
-    ctx.set_stream(torch.cuda.current_stream())
-    return ctx
+    return _bind(ctx)
 
 
 def dequantize_mxfp4(blocks: torch.Tensor, scales: torch.Tensor, rows: int, cols: int, *,
@@ -54,7 +62,7 @@ def dequantize_mxfp4(blocks: torch.Tensor, scales: torch.Tensor, rows: int, cols
         raise ValueError(f"unsupported scale dtype {scales.dtype}")
     c = context(ctx)
     if out is None:
-        out = torch.empty(max(rows * cols, 0), dtype=torch.int16, device=blocks.device)
+        out = blocks.new_empty(max(rows * cols, 0), dtype=torch.int16)
     st = c.lib.oxg_dequant_mxfp4(c.handle, blocks.data_ptr(), blocks.numel(), scales.data_ptr(),
                                  scales.numel(), fmt, rows, cols, out.data_ptr())
     if st == abi.OXG_ERR_SHAPE:
@@ -78,8 +86,7 @@ def device_context(x: torch.Tensor, ctx: abi.Context | None) -> abi.Context:
             ctx = _device_ctx[index] = abi.Context(index)
     elif ctx.device != index:
         raise ValueError(f"the context is on cuda:{ctx.device}, the input on {x.device}")
-    ctx.set_stream(torch.cuda.current_stream(index))
-    return ctx
+    return _bind(ctx)
 
 
 def check_status(status: int, ctx: abi.Context) -> None:
@@ -96,6 +103,8 @@ def rows_of(x: torch.Tensor, name: str) -> tuple[torch.Tensor, int, int]:
         raise ValueError(f"{name} must be a float32, bfloat16 or float16 CUDA tensor")
     if x.dim() == 0:
         raise ValueError(f"{name} must have at least one dimension")
+    if x.dim() == 2 and x.is_contiguous():
+        return x, x.shape[0], x.shape[1]
     if x.dim() != 2:
         x = x.reshape(-1, x.shape[-1]) if x.shape[-1] else x.reshape(0, 0)
     if x.shape[1] > 1 and x.stride(1) != 1 or x.shape[0] > 1 and x.stride(0) < x.shape[1]:
@@ -116,9 +125,8 @@ def quantized_like(x: torch.Tensor, cols: int, rows: int, tiled: bool) -> tuple[
     if tiled and x.dim() != 2:
         raise ValueError(f"tiled scales are those of one matrix: the input must have 2 dimensions, got {x.dim()}")
     lead = x.shape[:-1]
-    blocks = torch.empty(*lead, cols // 2, dtype=torch.uint8, device=x.device)
     shape = ((cols + 127) // 128, rows, 4) if tiled else (*lead, cols // 32)
-    return blocks, torch.empty(shape, dtype=torch.uint8, device=x.device)
+    return x.new_empty((*lead, cols // 2), dtype=torch.uint8), x.new_empty(shape, dtype=torch.uint8)
 
 
 def quantize_mxfp4(x: torch.Tensor, *, row_scale: torch.Tensor | None = None, scale_rule: str = "floor",
