@@ -18,6 +18,7 @@ struct Mx4QuantArgs {
   const void *x = nullptr;           // [rows, cols] (SwiGLU: [rows, 2 cols], gate and up interleaved)
   size_t ld = 0;                     // elements from one row to the next
   size_t rows = 0, cols = 0;         // of the quantised matrix; cols a multiple of 32
+  size_t scale_rows = 0;             // rows of the tiled scales (set by the launch)
   const float *row_scale = nullptr;  // [rows] factors, or null
   int rule = kMx4Floor;
   int tiled = 0;

@@ -11,8 +11,8 @@
 //
 // Bound: HBM. A thread owns 8 consecutive elements (one 16-byte load of 16-bit types, two of f32) and a
 // block is four neighbouring lanes, which share the largest magnitude by two shuffles; the codes leave as
-// one 4-byte word per thread. Each thread issues 64 bytes of loads, chunks a grid's width apart, before it works
-// on the first.
+// one 4-byte word per thread. Each thread issues 64 bytes of loads before it works on the first; a block takes
+// one contiguous run of chunks and ends.
 #include "common.cuh"
 #include "mx4.h"
 
@@ -116,11 +116,14 @@ __device__ __forceinline__ float min_nan(float a, float b) {
   asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
   return r;
 }
+__device__ __forceinline__ float max3_abs_nan(float a, float b, float c) {
+  float r;
+  asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
 // f32 bits of a block's largest magnitude (NaN if it holds one), shared by its four lanes
 __device__ __forceinline__ uint32_t block_top(const float (&v)[8]) {
-  float t = fabsf(v[0]);
-#pragma unroll
-  for (int i = 1; i < 8; ++i) t = max_nan(t, fabsf(v[i]));
+  float t = max3_abs_nan(max3_abs_nan(v[0], v[1], v[2]), max3_abs_nan(v[3], v[4], v[5]), max_nan(fabsf(v[6]), fabsf(v[7])));
   t = max_nan(t, __shfl_xor_sync(0xFFFFFFFFu, t, 1));
   return __float_as_uint(max_nan(t, __shfl_xor_sync(0xFFFFFFFFu, t, 2)));
 }
@@ -142,15 +145,16 @@ __device__ __forceinline__ double swiglu_f64(float gf, float uf, float alpha, fl
 }
 
 // Eight SwiGLU outputs from their gate / up pairs, quantised as the exact values would be. The f32 value comes
-// from the hardware's exponential and reciprocal (ten instructions instead of forty: with expf and the IEEE
-// quotient the kernel took 210 us for 32768 x 2880 from bf16). For g >= 2^-40 or 0 and x = -alpha g <= 40 its
-// relative error stays below kTol = 2^-17 = 128 2^-24: log2 e, -alpha log2 e and its product with g are rounded,
-// 2.5 2^-24 |x| in e^x; ex2 adds 2^-22, the reciprocal 2^-23, the sum, u + 1 and two products 2^-24 each, 110
-// 2^-24 in all. No intermediate leaves f32's normal range (|u + 1| is 0 or at least 2^-24, the sigmoid at least
-// e^-40 / 2). So where the block's largest magnitude or a scaled element lies within kTol of a border between
-// two scales or two codes (seen by rounding both (1 - kTol) and (1 + kTol) times the value), or where a gate lies
-// outside that range, the block's four lanes evaluate it again in f64: about 1 block in 300 of normally
-// distributed inputs. The codes then do not depend on which exponential computed them.
+// from the hardware's exponential and reciprocal (expf and the IEEE quotient: 210 us for 32768 x 2880 from bf16).
+// For x = -alpha g <= 40 its relative error stays below kTol = 2^-17 = 128 2^-24: log2 e, -alpha log2 e and its
+// product with g are rounded, 2.5 2^-24 |x| in e^x; ex2 adds 2^-22, the reciprocal 2^-23, the sum, u + 1 and two
+// products 2^-24 each, 110 2^-24 in all, as long as nothing leaves f32's normal range. What does is off by 2^-150
+// (1 + limit) at most, which is nothing to a block whose scale is 2^-100 or more while limit <= 2^18, and to
+// one that is zero throughout (its exact values lie below the smallest scale's first border). So where the
+// block's largest magnitude or a scaled element lies within kTol of a border between two scales or two codes
+// (the latter seen by rounding both (1 - kTol) and (1 + kTol) times the value), or where one of these conditions
+// does not hold, the block's four lanes evaluate it again in f64: about 1 block in 300 of normally distributed
+// inputs. The codes then do not depend on which exponential computed them.
 constexpr float kTol = 0x1p-17f;
 __device__ __forceinline__ uint32_t swiglu_quantize8_f64(const float (&gu)[16], float alpha, float limit, int rule, int *byte,
                                                       uint32_t lanes) {
@@ -184,28 +188,31 @@ __device__ __forceinline__ uint32_t swiglu_quantize8_f64(const float (&gu)[16], 
 }
 __device__ __forceinline__ uint32_t swiglu_quantize8(const float (&gu)[16], float alpha, float limit, int rule, int *byte) {
   const float c = -alpha * 1.4426950408889634f;  // e^(-alpha g) = 2^(c g)
-  float h[8];
-  bool close = false;
+  float h[8], sum = 0.f;
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     const float g = min_nan(gu[2 * i], limit), u = max_nan(min_nan(gu[2 * i + 1], limit), -limit);
-    const float x = c * g;
     float e, r;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(x));
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(c * g));
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + e));
     h[i] = g * r * (u + 1.0f);
-    close |= x > 57.f || (fabsf(g) < 0x1p-40f && g != 0.f);  // 40 log2 e
+    sum += e;
+  }
+  bool close = sum > 0x1p57f;  // some x beyond 40 (40 log2 e > 57)
+  if (!(limit <= 0x1p18f)) {   // without a clamp that means something, every gate that is neither 0 nor ordinary
+#pragma unroll
+    for (int i = 0; i < 8; ++i) close |= fabsf(gu[2 * i]) < 0x1p-40f && gu[2 * i] != 0.f;
   }
   const uint32_t top = block_top(h);
   const bool finite = top < 0x7F800000u;
-  close |= top == 0x7F800000u;  // an overflow, perhaps only of the f32 arithmetic
-  const float t = __uint_as_float(top);
+  close |= top == 0x7F800000u;            // an overflow, perhaps only of the f32 arithmetic
+  close |= top - 1u < (29u << 23) - 1u;   // scales below 2^-100, but for a block of zeros
+  close |= ((top + 128u) & 0x3FFFFFu) < 256u;  // within 128 2^-23 of a power of two or of 1.5 times one
   *byte = finite ? scale_byte(top, rule) : 255;
   const float inv = inverse_scale(finite ? *byte : 1);
-  const uint32_t w = pack_scaled(h, inv * (1.0f - kTol)), w1 = pack_scaled(h, inv * (1.0f + kTol));
-  close |= w != w1 || scale_byte(__float_as_uint(t * (1.0f - kTol)), rule) != scale_byte(__float_as_uint(t * (1.0f + kTol)), rule);
-  const int lane = threadIdx.x & 31;
-  const uint32_t lanes = 0xFu << (lane & ~3);
+  const uint32_t w = pack_scaled(h, inv * (1.0f - kTol));
+  close |= w != pack_scaled(h, inv * (1.0f + kTol));
+  const uint32_t lanes = 0xFu << (threadIdx.x & 28);
   if ((__ballot_sync(0xFFFFFFFFu, close) & lanes) != 0u)  // the four lanes of a block go together
     return swiglu_quantize8_f64(gu, alpha, limit, rule, byte, lanes);
   return finite ? w : 0u;
@@ -234,57 +241,54 @@ struct Div {
 enum Lay { kFlat, kGrid, kAny };
 
 template <int T, bool SWIGLU, Lay LAY, int UNR>
-__global__ void __launch_bounds__(kThreads) mx4_quantize_kernel(const Mx4QuantArgs a, size_t n_chunks, const Div per_row) {
+__global__ void __launch_bounds__(kThreads) mx4_quantize_kernel(const Mx4QuantArgs a, uint32_t n_chunks, const Div per_row) {
   constexpr int N = SWIGLU ? 16 : 8;
-  const size_t stride = (size_t)gridDim.x * kThreads;
-  // every lane of a warp makes the same rounds (shuffles below); chunks come in fours, so blocks stay whole
-  for (size_t c0 = (size_t)blockIdx.x * kThreads + threadIdx.x; c0 - (threadIdx.x & 31) < n_chunks; c0 += UNR * stride) {
-    Raw<T, N, LAY != kAny> raw[UNR];
-    size_t row[UNR];
-    uint32_t col[UNR];
+  // every lane of a warp goes through the shuffles below; chunks come in fours, so blocks stay whole
+  const uint32_t c0 = blockIdx.x * (UNR * kThreads) + threadIdx.x;
+  Raw<T, N, LAY != kAny> raw[UNR];
+  uint32_t row[UNR], col[UNR];
 #pragma unroll
-    for (int u = 0; u < UNR; ++u) {
-      const size_t c = c0 + u * stride;
-      if (LAY != kFlat) {
-        row[u] = n_chunks <= 0xFFFFFFFFull ? per_row.quotient((uint32_t)c) : c / per_row.d;
-        col[u] = (uint32_t)(c - row[u] * per_row.d);
-      }
-      const size_t at = LAY == kFlat ? c * N : row[u] * a.ld + (size_t)col[u] * N;
-      if (c < n_chunks)
-        raw[u].load(static_cast<const uint8_t *>(a.x) + at * Elem<T>::kBytes);
-      else
-#pragma unroll
-        for (int i = 0; i < Raw<T, N, LAY != kAny>::kWords; ++i) raw[u].w[i] = make_uint4(0u, 0u, 0u, 0u);
+  for (int u = 0; u < UNR; ++u) {
+    const uint32_t c = c0 + u * kThreads;
+    if (LAY != kFlat) {
+      row[u] = per_row.quotient(c);
+      col[u] = c - row[u] * per_row.d;
     }
+    const size_t at = LAY == kFlat ? (size_t)c * N : row[u] * a.ld + (size_t)col[u] * N;
+    if (c < n_chunks)
+      raw[u].load(static_cast<const uint8_t *>(a.x) + at * Elem<T>::kBytes);
+    else
 #pragma unroll
-    for (int u = 0; u < UNR; ++u) {
-      const size_t c = c0 + u * stride;
-      float v[N];
-      raw[u].values(v);
-      int byte;
-      uint32_t w;
-      if constexpr (SWIGLU) {
-        w = swiglu_quantize8(v, a.alpha, a.limit, a.rule, &byte);
-      } else {
-        if (LAY != kFlat && a.row_scale) {
-          const float f = c < n_chunks ? __ldg(a.row_scale + row[u]) : 0.f;
+      for (int i = 0; i < Raw<T, N, LAY != kAny>::kWords; ++i) raw[u].w[i] = make_uint4(0u, 0u, 0u, 0u);
+  }
 #pragma unroll
-          for (int i = 0; i < N; ++i) v[i] = __fmul_rn(v[i], f);
-        }
-        w = quantize8(v, a.rule, &byte);
+  for (int u = 0; u < UNR; ++u) {
+    const uint32_t c = c0 + u * kThreads;
+    float v[N];
+    raw[u].values(v);
+    int byte;
+    uint32_t w;
+    if constexpr (SWIGLU) {
+      w = swiglu_quantize8(v, a.alpha, a.limit, a.rule, &byte);
+    } else {
+      if (LAY != kFlat && a.row_scale) {
+        const float f = c < n_chunks ? __ldg(a.row_scale + row[u]) : 0.f;
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[i] = __fmul_rn(v[i], f);
       }
-      if (c >= n_chunks) continue;
-      reinterpret_cast<uint32_t *>(a.blocks)[c] = w;
-      if ((c & 3) == 0) {
-        if (LAY == kFlat || !a.tiled) {
-          a.scales[c >> 2] = (uint8_t)byte;
-        } else {
-          const uint32_t kb = col[u] >> 2;
-          uint8_t *d = a.scales + ((size_t)(kb >> 2) * a.rows + row[u]) * 4;
-          d[kb & 3] = (uint8_t)byte;
-          if (col[u] + 4 == per_row.d)  // zero where the row ends inside a 128-element stretch
-            for (uint32_t j = (kb & 3) + 1; j < 4; ++j) d[j] = 0;
-        }
+      w = quantize8(v, a.rule, &byte);
+    }
+    if (c >= n_chunks) continue;
+    reinterpret_cast<uint32_t *>(a.blocks)[c] = w;
+    if ((c & 3) == 0) {
+      if (LAY == kFlat || !a.tiled) {
+        a.scales[c >> 2] = (uint8_t)byte;
+      } else {
+        const uint32_t kb = col[u] >> 2;
+        uint8_t *d = a.scales + ((size_t)(kb >> 2) * a.scale_rows + row[u]) * 4;
+        d[kb & 3] = (uint8_t)byte;
+        if (col[u] + 4 == per_row.d)  // zero where the row ends inside a 128-element stretch
+          for (uint32_t j = (kb & 3) + 1; j < 4; ++j) d[j] = 0;
       }
     }
   }
@@ -307,19 +311,31 @@ __global__ void __launch_bounds__(kThreads)
 }
 
 template <int T, bool SWIGLU, Lay LAY, int UNR>
-cudaError_t launch_unr(const Mx4QuantArgs &a, size_t n_chunks, int n_sms, cudaStream_t stream) {
-  const size_t want = (n_chunks + (size_t)kThreads * UNR - 1) / ((size_t)kThreads * UNR), cap = (size_t)n_sms * 8;
-  mx4_quantize_kernel<T, SWIGLU, LAY, UNR><<<(unsigned)(want < cap ? want : cap), kThreads, 0, stream>>>(
+cudaError_t launch_unr(const Mx4QuantArgs &a, cudaStream_t stream) {
+  const uint32_t n_chunks = (uint32_t)(a.rows * (a.cols / 8));
+  mx4_quantize_kernel<T, SWIGLU, LAY, UNR><<<(n_chunks + UNR * kThreads - 1) / (UNR * kThreads), kThreads, 0, stream>>>(
       a, n_chunks, Div((uint32_t)(a.cols / 8)));
   return cudaGetLastError();
 }
 template <int T, bool SWIGLU, Lay LAY>
-cudaError_t launch_lay(const Mx4QuantArgs &a, int n_sms, cudaStream_t stream) {
-  const size_t n_chunks = a.rows * (a.cols / 8);
-  // chunks per thread in flight: 64 bytes of loads, once there is a chunk for every thread that fits the GPU
+cudaError_t launch_lay(Mx4QuantArgs a, int n_sms, cudaStream_t stream) {
+  // 64 bytes of loads in flight per thread, once there is a chunk for every thread that fits the GPU
   constexpr int UNR = 4 / (Elem<T>::kBytes / 2) / (SWIGLU ? 2 : 1);
-  if (n_chunks <= (size_t)n_sms * 2048) return launch_unr<T, SWIGLU, LAY, 1>(a, n_chunks, n_sms, stream);
-  return launch_unr<T, SWIGLU, LAY, UNR>(a, n_chunks, n_sms, stream);
+  const size_t width = a.cols * (SWIGLU ? 2 : 1) * Elem<T>::kBytes;
+  // 32-bit chunk numbers: a kernel takes the rows of at most 2^31 chunks (34 GB of bf16)
+  const size_t most = ((size_t)1 << 31) / (a.cols / 8), rows = a.rows;
+  a.scale_rows = rows;
+  for (size_t r = 0; r < rows; r += most) {
+    a.rows = rows - r < most ? rows - r : most;
+    const cudaError_t st = a.rows * (a.cols / 8) <= (size_t)n_sms * 2048 ? launch_unr<T, SWIGLU, LAY, 1>(a, stream)
+                                                                        : launch_unr<T, SWIGLU, LAY, UNR>(a, stream);
+    if (st) return st;
+    a.x = static_cast<const uint8_t *>(a.x) + a.rows * (a.ld * Elem<T>::kBytes > width ? a.ld * Elem<T>::kBytes : width);
+    a.blocks += a.rows * (a.cols / 2);
+    a.scales += a.rows * (a.tiled ? 4 : a.cols / 32);
+    if (a.row_scale) a.row_scale += a.rows;
+  }
+  return cudaSuccess;
 }
 template <int T, bool SWIGLU>
 cudaError_t launch_op(const Mx4QuantArgs &a, int n_sms, cudaStream_t stream) {
