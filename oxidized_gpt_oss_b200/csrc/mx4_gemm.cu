@@ -80,7 +80,7 @@ struct Params {
   int words;        // scale words per row
   int box;          // activation rows per TMA box
   int out_bf16;
-  int pair_stores;  // bf16 rows start on 4-byte boundaries
+  int pair_stores;  // bf16: n is even and rows start on 4-byte boundaries
   int *err;
 };
 
@@ -450,7 +450,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const bool in = f < p.n;
       const float bias = p.bias && in && !SPLIT ? bf16_to_f32(__ldg(p.bias + (size_t)t.g * p.n + f)) : 0.f;
       const uint32_t base = tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)(buf * C::NMAX);
-      const bool whole = t.f0 + kTileW <= p.n && p.pair_stores;  // no feature of the tile is missing
+      const bool whole = t.f0 + kTileW <= p.n;
       for (int c0 = 32 * half; c0 < t.rows; c0 += 64) {
         uint32_t v[32];
         tmem_ld_32_async(base + (uint32_t)c0, v);
@@ -459,50 +459,48 @@ __global__ void __launch_bounds__(kThreads, 1)
           // this part of K: [column][feature], where the stages were (all of them have been read)
           float *part = reinterpret_cast<float *>(stages) + c0 * kTileW + q * 32 + lane;
 #pragma unroll
-          for (int i = 0; i < 32; ++i)
-            if (c0 + i < t.rows) part[i * kTileW] = __uint_as_float(v[i]);
-        } else if (p.out_bf16 && whole && c0 + 32 <= t.rows) {
+          for (int i = 0; i < 32; ++i) part[i * kTileW] = __uint_as_float(v[i]);
+        } else if (p.out_bf16 && p.pair_stores) {
           // lanes 2i and 2i + 1 trade halves: the even one stores both features of an even column, the odd
-          // one of an odd column, 4 bytes each
-          const int odd = lane & 1;
+          // one of an odd column, 4 bytes each (n is even, so both exist or neither does)
+          const int odd = lane & 1, lim = in ? t.rows - c0 - odd : 0;
+          const size_t two = 2 * p.ldo;
           uint16_t *o = static_cast<uint16_t *>(p.out) + (size_t)(t.row0 + c0 + odd) * p.ldo + (f - odd);
           float other[16];
 #pragma unroll
           for (int i = 0; i < 16; ++i)
             other[i] = __shfl_xor_sync(0xFFFFFFFFu, __uint_as_float(odd ? v[2 * i] : v[2 * i + 1]) + bias, 1);
+          uint32_t both[16];
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
             const float mine = __uint_as_float(odd ? v[2 * i + 1] : v[2 * i]) + bias;
-            *reinterpret_cast<uint32_t *>(o) = odd ? pack_bf16x2(other[i], mine) : pack_bf16x2(mine, other[i]);
-            o += 2 * p.ldo;
+            both[i] = odd ? pack_bf16x2(other[i], mine) : pack_bf16x2(mine, other[i]);
           }
-        } else if (!p.out_bf16 && t.f0 + kTileW <= p.n && c0 + 32 <= t.rows) {
-          float *o = static_cast<float *>(p.out) + (size_t)(t.row0 + c0) * p.ldo + f;
+          if (whole && c0 + 32 <= t.rows) {
 #pragma unroll
-          for (int i = 0; i < 32; ++i) {
-            *o = __uint_as_float(v[i]) + bias;
-            o += p.ldo;
+            for (int i = 0; i < 16; ++i, o += two) *reinterpret_cast<uint32_t *>(o) = both[i];
+          } else {
+#pragma unroll
+            for (int i = 0; i < 16; ++i, o += two)
+              if (2 * i < lim) *reinterpret_cast<uint32_t *>(o) = both[i];
           }
-        } else if (!p.out_bf16) {
-          float *o = static_cast<float *>(p.out) + (size_t)(t.row0 + c0) * p.ldo + f;
-#pragma unroll
-          for (int i = 0; i < 32; ++i)
-            if (in && c0 + i < t.rows) o[(size_t)i * p.ldo] = __uint_as_float(v[i]) + bias;
         } else {
-          const int odd = lane & 1, fe = f - odd;
-          uint16_t *o = static_cast<uint16_t *>(p.out) + (size_t)(t.row0 + c0 + odd) * p.ldo + fe;
+          const int lim = in ? t.rows - c0 : 0;
+          const size_t o = (size_t)(t.row0 + c0) * p.ldo + f;
+          if (p.out_bf16) {
+            uint16_t *d = static_cast<uint16_t *>(p.out) + o;
 #pragma unroll
-          for (int i = 0; i < 32; i += 2) {
-            const float v0 = __uint_as_float(v[i]) + bias, v1 = __uint_as_float(v[i + 1]) + bias;
-            const float other = __shfl_xor_sync(0xFFFFFFFFu, odd ? v0 : v1, 1);
-            const uint32_t both = pack_bf16x2(odd ? other : v0, odd ? v1 : other);
-            if (c0 + i + odd >= t.rows) continue;
-            uint16_t *dst = o + (size_t)i * p.ldo;
-            if (fe + 1 < p.n && p.pair_stores) {
-              *reinterpret_cast<uint32_t *>(dst) = both;
+            for (int i = 0; i < 32; ++i, d += p.ldo)
+              if (i < lim) *d = (uint16_t)pack_bf16x2(__uint_as_float(v[i]) + bias, 0.f);
+          } else {
+            float *d = static_cast<float *>(p.out) + o;
+            if (whole && c0 + 32 <= t.rows) {
+#pragma unroll
+              for (int i = 0; i < 32; ++i, d += p.ldo) *d = __uint_as_float(v[i]) + bias;
             } else {
-              if (fe < p.n) dst[0] = (uint16_t)both;
-              if (fe + 1 < p.n) dst[1] = (uint16_t)(both >> 16);
+#pragma unroll
+              for (int i = 0; i < 32; ++i, d += p.ldo)
+                if (i < lim) *d = __uint_as_float(v[i]) + bias;
             }
           }
         }
@@ -648,7 +646,7 @@ cudaError_t launch_mx4_gemm(const Mx4GemmArgs &a, int n_sms, cudaStream_t stream
   p.k_steps = (a.k + kStageK - 1) / kStageK;
   p.words = (a.k + 127) / 128;
   p.out_bf16 = a.out_bf16;
-  p.pair_stores = a.ldo % 2 == 0 && (uintptr_t)a.out % 4 == 0;
+  p.pair_stores = a.n % 2 == 0 && (a.ldo % 2 == 0 || a.m == 1) && (uintptr_t)a.out % 4 == 0;
   p.err = a.err;
   if ((long long)a.m > 64ll * a.groups) return launch_cfg<Pair>(a, p, n_sms, 1, stream);
   const long long tiles = ((long long)a.n + kTileW - 1) / kTileW * std::min(a.groups, a.m);
