@@ -9,6 +9,15 @@
 
 namespace oxg {
 
+#ifdef __CUDACC__
+// The MXFP4 kernels are launched as programmatic dependents and let their own dependents start at once: the next
+// one's launch and setup then overlap this one's end. Every thread that touches memory which an earlier kernel
+// may have written, or writes any, first waits for all of the earlier kernel; through that kernel's own wait
+// this covers every kernel before it.
+__device__ __forceinline__ void launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void wait_prerequisites() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+#endif
+
 // Element types and scale rules and layouts, as the public header numbers them.
 enum { kMx4F32 = 0, kMx4Bf16 = 1, kMx4F16 = 2 };
 enum { kMx4Floor = 0, kMx4NoClip = 1 };

@@ -156,7 +156,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   constexpr int STAGES = C::STAGES;
   extern __shared__ uint8_t smem_raw[];
   uint8_t *stages = smem_raw + ((1024u - (smem_addr(smem_raw) & 1023u)) & 1023u);
-  __shared__ uint64_t full_[STAGES], scaled_[STAGES], empty_[STAGES];
+  __shared__ uint64_t full_[STAGES], empty_[STAGES];
   __shared__ uint64_t acc_full[2], acc_empty[2], mma_done;
   __shared__ uint32_t tmem_slot;
   __shared__ int tile0_[kMx4MaxGroups + 1], row0_[kMx4MaxGroups + 1];
@@ -167,8 +167,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (SPLIT) asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(n_ranks));
   if (threadIdx.x == 0) {
     for (int s = 0; s < STAGES; ++s) {
-      mbar_init(&full_[s], 1);
-      mbar_init(&scaled_[s], 2 * C::CTAS);
+      mbar_init(&full_[s], 1 + 2 * C::CTAS);  // the codes' bytes, and both operands' scales in each CTA
       mbar_init(&empty_[s], 1);
     }
     for (int b = 0; b < 2; ++b) {
@@ -187,6 +186,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       tmem_relinquish();
     }
   }
+  launch_dependents();
+  wait_prerequisites();  // nothing above touches memory that an earlier kernel writes
   if (warp == 2) {  // running sums of the groups' rows and activation tiles
     int rows_run = 0, tiles_run = 0;
     for (int g0 = 0; g0 < p.groups; g0 += 32) {
@@ -306,10 +307,11 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
     }
     if (!ok && (rank == 0 || SPLIT)) {
-      // copies in flight land before the CTA (pair) ends: stages below s have been loaded in this round
+      // copies in flight land before the CTA (pair) ends: stages below s have been loaded in this round. A
+      // barrier whose scales never came costs one full wait, long after any copy has landed.
       for (int i = 0; i < STAGES; ++i) {
         const int last = i < s ? round : round - 1;
-        if (last >= 0) mbar_wait(&full_[i], last & 1, p.err, kMx4ErrWait);
+        if (last >= 0 && !mbar_wait(&full_[i], last & 1, p.err, kMx4ErrWait)) break;
       }
     }
   } else if (warp == 1) {
@@ -327,7 +329,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         const uint32_t d = tmem + (uint32_t)(buf * C::NMAX);
         const uint32_t id0 = idesc_mxf4(kTileW * C::CTAS, cols, 0), id2 = idesc_mxf4(kTileW * C::CTAS, cols, 2);
         for (int ks = k_lo; ks < k_hi; ++ks) {
-          if (!(ok = mbar_wait(&scaled_[s], phase, p.err, kMx4ErrWait) && mbar_wait(&full_[s], phase, p.err, kMx4ErrWait))) break;
+          if (!(ok = mbar_wait(&full_[s], phase, p.err, kMx4ErrWait))) break;
           tc_fence_after();
           if (elect_one()) {
             const uint32_t st = smem_addr(stages + s * C::BYTES), sf = st + kWBytes + C::X_BYTES;
@@ -425,8 +427,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) {
-          if (PAIR) mbar_arrive_cluster(rank0(&scaled_[s]));
-          else mbar_arrive(&scaled_[s]);
+          if (PAIR) mbar_arrive_cluster(rank0(&full_[s]));
+          else mbar_arrive(&full_[s]);
         }
         fetch();
         if ((s += kScaleWarps) >= STAGES) {
@@ -602,15 +604,17 @@ cudaError_t launch_cfg(const Mx4GemmArgs &a, Params &p, int n_sms, int ranks, cu
     if (dev < 64) ready.fetch_or(1ull << dev, std::memory_order_relaxed);
   }
   cudaLaunchConfig_t cfg{};
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = (unsigned)(C::SPLIT ? ranks : C::CTAS);
-  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = (unsigned)(C::SPLIT ? ranks : C::CTAS);
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
   cfg.blockDim = dim3(kThreads);
   cfg.dynamicSmemBytes = C::SMEM;
   cfg.stream = stream;
   cfg.attrs = attr;
-  cfg.numAttrs = C::SPLIT || C::PAIR ? 1 : 0;
+  cfg.numAttrs = C::SPLIT || C::PAIR ? 2 : 1;
   long long at_once = n_sms;  // tiles in work side by side; the GPU's clusters may not hold every SM
   if (C::PAIR) {
     static const int pairs = [&] {

@@ -243,6 +243,8 @@ enum Lay { kFlat, kGrid, kAny };
 template <int T, bool SWIGLU, Lay LAY, int UNR>
 __global__ void __launch_bounds__(kThreads) mx4_quantize_kernel(const Mx4QuantArgs a, uint32_t n_chunks, const Div per_row) {
   constexpr int N = SWIGLU ? 16 : 8;
+  launch_dependents();
+  wait_prerequisites();
   // every lane of a warp goes through the shuffles below; chunks come in fours, so blocks stay whole
   const uint32_t c0 = blockIdx.x * (UNR * kThreads) + threadIdx.x;
   Raw<T, N, LAY != kAny> raw[UNR];
@@ -298,6 +300,8 @@ __global__ void __launch_bounds__(kThreads) mx4_quantize_kernel(const Mx4QuantAr
 __global__ void __launch_bounds__(kThreads)
     mx4_tile_scales_kernel(const uint8_t *__restrict__ src, size_t n_words, size_t rows, uint32_t kb, uint32_t words,
                            uint32_t *__restrict__ dst) {
+  launch_dependents();
+  wait_prerequisites();
   for (size_t i = (size_t)blockIdx.x * kThreads + threadIdx.x; i < n_words; i += (size_t)gridDim.x * kThreads) {
     const size_t r = i % rows, q = i / rows, g = q / words;
     const uint32_t b0 = (uint32_t)(q - g * words) * 4;
@@ -310,12 +314,24 @@ __global__ void __launch_bounds__(kThreads)
   }
 }
 
+template <class... P, class... A>
+cudaError_t launch_dependent(void (*kernel)(P...), unsigned grid, cudaStream_t stream, A... args) {
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(kThreads);
+  cfg.stream = stream;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, P(args)...);
+}
 template <int T, bool SWIGLU, Lay LAY, int UNR>
 cudaError_t launch_unr(const Mx4QuantArgs &a, cudaStream_t stream) {
   const uint32_t n_chunks = (uint32_t)(a.rows * (a.cols / 8));
-  mx4_quantize_kernel<T, SWIGLU, LAY, UNR><<<(n_chunks + UNR * kThreads - 1) / (UNR * kThreads), kThreads, 0, stream>>>(
-      a, n_chunks, Div((uint32_t)(a.cols / 8)));
-  return cudaGetLastError();
+  return launch_dependent(mx4_quantize_kernel<T, SWIGLU, LAY, UNR>, (n_chunks + UNR * kThreads - 1) / (UNR * kThreads), stream,
+                          a, n_chunks, Div((uint32_t)(a.cols / 8)));
 }
 template <int T, bool SWIGLU, Lay LAY>
 cudaError_t launch_lay(Mx4QuantArgs a, int n_sms, cudaStream_t stream) {
@@ -363,9 +379,8 @@ cudaError_t launch_mx4_tile_scales(const uint8_t *src, size_t groups, size_t row
   const size_t n_words = groups * rows * words;
   if (n_words == 0) return cudaSuccess;
   const size_t want = (n_words + kThreads - 1) / kThreads, cap = (size_t)n_sms * 16;
-  mx4_tile_scales_kernel<<<(unsigned)(want < cap ? want : cap), kThreads, 0, stream>>>(src, n_words, rows, kb, words,
-                                                                                       reinterpret_cast<uint32_t *>(dst));
-  return cudaGetLastError();
+  return launch_dependent(mx4_tile_scales_kernel, (unsigned)(want < cap ? want : cap), stream, src, n_words, rows, kb, words,
+                          reinterpret_cast<uint32_t *>(dst));
 }
 
 }  // namespace oxg
