@@ -159,6 +159,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   __shared__ uint64_t full_[STAGES], empty_[STAGES];
   __shared__ uint64_t acc_full[2], acc_empty[2], mma_done;
   __shared__ uint32_t tmem_slot;
+  __shared__ int cols_[STAGES];  // the MMA's N for a stage's tile, from the TMA warp
   __shared__ int tile0_[kMx4MaxGroups + 1], row0_[kMx4MaxGroups + 1];
 
   const int warp = __shfl_sync(0xFFFFFFFFu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
@@ -278,8 +279,10 @@ __global__ void __launch_bounds__(kThreads, 1)
     __syncwarp();
     int s = 0, round = 0;
     bool ok = true;
+    Tile next{};
+    if (item0 < total) next = tile_at(item0);
     for (int item = item0; ok && item < total; item += step) {
-      const Tile t = tile_at(item);
+      const Tile t = next;
       const int half = t.cols / C::CTAS, boxes = (half + p.box - 1) / p.box;
       const int x0 = t.row0 + (PAIR ? (int)rank * half : 0);
       const uint32_t tx = (uint32_t)(C::CTAS * (kWBytes + boxes * p.box * 128));
@@ -287,6 +290,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (round > 0 && !(ok = mbar_wait(&empty_[s], (round - 1) & 1, p.err, kMx4ErrWait))) break;
         if (elect_one()) {
           uint8_t *st = stages + s * C::BYTES;
+          cols_[s] = t.cols;
           if (rank == 0 || SPLIT) mbar_arrive_expect_tx(&full_[s], tx);
           if (PAIR) {
             const uint32_t bar = mapa_shared(smem_addr(&full_[s]), 0);
@@ -300,6 +304,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
         }
         __syncwarp();
+        if (ks == k_lo && item + step < total) next = tile_at(item + step);  // while the ring is full
         if (++s == STAGES) {
           s = 0;
           ++round;
@@ -320,17 +325,20 @@ __global__ void __launch_bounds__(kThreads, 1)
       int s = 0, phase = 0, j = 0;
       bool ok = true;
       const uint32_t sfw = tmem + C::SFW_COL, sfx = tmem + C::SFX_COL;
-      int next_cols = item0 < total ? tile_at(item0).cols : 0;
       for (int item = item0; ok && item < total; item += step, ++j) {
-        const int cols = next_cols;
         const int buf = j & 1, rr = j >> 1;
         if (rr > 0 && !(ok = mbar_wait(&acc_empty[buf], (rr - 1) & 1, p.err, kMx4ErrWait))) break;
         tc_fence_after();
         const uint32_t d = tmem + (uint32_t)(buf * C::NMAX);
-        const uint32_t id0 = idesc_mxf4(kTileW * C::CTAS, cols, 0), id2 = idesc_mxf4(kTileW * C::CTAS, cols, 2);
+        uint32_t id0 = 0, id2 = 0;
         for (int ks = k_lo; ks < k_hi; ++ks) {
           if (!(ok = mbar_wait(&full_[s], phase, p.err, kMx4ErrWait))) break;
           tc_fence_after();
+          if (ks == k_lo) {  // where a tile lies takes longer to work out than the tensor cores have work in hand
+            const int cols = cols_[s];
+            id0 = idesc_mxf4(kTileW * C::CTAS, cols, 0);
+            id2 = idesc_mxf4(kTileW * C::CTAS, cols, 2);
+          }
           if (elect_one()) {
             const uint32_t st = smem_addr(stages + s * C::BYTES), sf = st + kWBytes + C::X_BYTES;
             const int mmas = (p.k - ks * kStageK + 63) / 64;  // 4, but for the end of K
@@ -363,8 +371,6 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
           }
           __syncwarp();
-          // the next tile's width while the tensor cores have work in hand, not between the two tiles
-          if (ks == k_lo && item + step < total) next_cols = tile_at(item + step).cols;
           if (++s == STAGES) {
             s = 0;
             phase ^= 1;
