@@ -143,10 +143,9 @@ __device__ __forceinline__ bool elect_one() {
   return p != 0;
 }
 
-// A CTA's way through its tiles' stages.
-struct Cursor {
-  int item, ks;
-  Tile t;
+// A CTA's way through its tiles: item = xt * n_tiles + wt, the wt-th weight tile of activation tile xt (of group g).
+struct Walk {
+  int item, xt, wt, g;
 };
 
 template <class C>
@@ -160,7 +159,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   __shared__ uint64_t acc_full[2], acc_empty[2], mma_done;
   __shared__ uint32_t tmem_slot;
   __shared__ int cols_[STAGES];  // the MMA's N for a stage's tile, from the TMA warp
-  __shared__ int tile0_[kMx4MaxGroups + 1], row0_[kMx4MaxGroups + 1];
+  __shared__ int tile0_[kMx4MaxGroups + 1], row0_[kMx4MaxGroups + 1], per_[kMx4MaxGroups];  // per: rows of a group's tiles
 
   const int warp = __shfl_sync(0xFFFFFFFFu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
   const uint32_t rank = PAIR || SPLIT ? cluster_ctarank() : 0u;
@@ -208,6 +207,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       // counts beyond the rows there are: the groups end with the rows
       const int first = (int)min(r - c, (long long)p.m), last = (int)min(r, (long long)p.m);
       int t = (last - first + C::NMAX - 1) / C::NMAX;
+      const int per = round_cols<C>((last - first + max(t, 1) - 1) / max(t, 1));  // equal tiles
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
         const int u = __shfl_up_sync(0xFFFFFFFFu, t, o);
@@ -215,6 +215,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       if (g < p.groups) {
         row0_[g + 1] = last;
+        per_[g] = per;
         tile0_[g + 1] = tiles_run + t;
       }
       rows_run = __shfl_sync(0xFFFFFFFFu, last, 31);
@@ -234,39 +235,47 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int k_lo = SPLIT ? (int)((long long)p.k_steps * rank / n_ranks) : 0;
   const int k_hi = SPLIT ? (int)((long long)p.k_steps * (rank + 1) / n_ranks) : p.k_steps;
 
-  auto tile_at = [&](int item) {
-    const int xt = item / p.n_tiles;
-    int lo = 0, hi = p.groups;  // the last group that starts at or before xt: empty ones before it start there too
+  const int step_x = step / p.n_tiles, step_w = step - step_x * p.n_tiles;
+
+  // the last group from g on that starts at or before xt: empty ones before it start there too
+  auto group_of = [&](int g, int xt) {
+    if (tile0_[g + 1] > xt) return g;
+    int lo = g, hi = p.groups;
     while (hi - lo > 1) {
       const int mid = (lo + hi) >> 1;
       if (tile0_[mid] <= xt) lo = mid;
       else hi = mid;
     }
-    const int first = row0_[lo], rows = row0_[lo + 1] - first, nt = tile0_[lo + 1] - tile0_[lo];
-    const int per = round_cols<C>((rows + nt - 1) / nt);  // equal tiles
+    return lo;
+  };
+  auto start = [&] {
+    Walk w;
+    w.item = item0;
+    w.xt = item0 / p.n_tiles;
+    w.wt = item0 - w.xt * p.n_tiles;
+    w.g = item0 < total ? group_of(0, w.xt) : 0;
+    return w;
+  };
+  auto advance = [&](Walk &w) {
+    w.item += step;
+    w.xt += step_x;
+    w.wt += step_w;
+    if (w.wt >= p.n_tiles) {
+      w.wt -= p.n_tiles;
+      ++w.xt;
+    }
+    if (w.item < total) w.g = group_of(w.g, w.xt);
+  };
+  auto tile_of = [&](const Walk &w) {
+    const int first = row0_[w.g], rows = row0_[w.g + 1] - first, per = per_[w.g];
+    const int i0 = (w.xt - tile0_[w.g]) * per;
     Tile t;
-    t.g = lo;
-    t.f0 = (item - xt * p.n_tiles) * (kTileW * C::CTAS) + (PAIR ? (int)rank * kTileW : 0);
-    const int i0 = (xt - tile0_[lo]) * per;
+    t.g = w.g;
+    t.f0 = w.wt * (kTileW * C::CTAS) + (PAIR ? (int)rank * kTileW : 0);
     t.row0 = first + i0;
     t.rows = min(per, rows - i0);
     t.cols = round_cols<C>(t.rows);
     return t;
-  };
-  auto start = [&] {
-    Cursor c;
-    c.item = item0;
-    c.ks = k_lo;
-    if (item0 < total) c.t = tile_at(item0);
-    return c;
-  };
-  auto advance = [&](Cursor &c, int by) {
-    c.ks += by;
-    while (c.ks >= k_hi && c.item < total) {
-      c.ks -= k_hi - k_lo;
-      c.item += step;
-      if (c.item < total) c.t = tile_at(c.item);
-    }
   };
   auto rank0 = [&](uint64_t *bar) { return PAIR ? mapa_shared(smem_addr(bar), 0) : smem_addr(bar); };
 
@@ -279,10 +288,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     __syncwarp();
     int s = 0, round = 0;
     bool ok = true;
-    Tile next{};
-    if (item0 < total) next = tile_at(item0);
-    for (int item = item0; ok && item < total; item += step) {
-      const Tile t = next;
+    for (Walk w = start(); ok && w.item < total; advance(w)) {
+      const Tile t = tile_of(w);
       const int half = t.cols / C::CTAS, boxes = (half + p.box - 1) / p.box;
       const int x0 = t.row0 + (PAIR ? (int)rank * half : 0);
       const uint32_t tx = (uint32_t)(C::CTAS * (kWBytes + boxes * p.box * 128));
@@ -304,7 +311,6 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
         }
         __syncwarp();
-        if (ks == k_lo && item + step < total) next = tile_at(item + step);  // while the ring is full
         if (++s == STAGES) {
           s = 0;
           ++round;
@@ -334,7 +340,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int ks = k_lo; ks < k_hi; ++ks) {
           if (!(ok = mbar_wait(&full_[s], phase, p.err, kMx4ErrWait))) break;
           tc_fence_after();
-          if (ks == k_lo) {  // where a tile lies takes longer to work out than the tensor cores have work in hand
+          if (ks == k_lo) {
             const int cols = cols_[s];
             id0 = idesc_mxf4(kTileW * C::CTAS, cols, 0);
             id2 = idesc_mxf4(kTileW * C::CTAS, cols, 2);
@@ -396,21 +402,33 @@ __global__ void __launch_bounds__(kThreads, 1)
       constexpr bool X = decltype(xs_)::value;
       constexpr int Q = X ? XQ : 4;
       uint32_t v[2][Q];  // the words of this warp's next stage
-      Cursor c = start();
-      advance(c, first);
+      Walk at = start();
+      Tile t{};
+      if (at.item < total) t = tile_of(at);
+      int ks = k_lo;
+      auto skip = [&](int stages) {
+        ks += stages;
+        if (ks < k_hi) return;
+        while (ks >= k_hi && at.item < total) {
+          ks -= k_hi - k_lo;
+          advance(at);
+        }
+        if (at.item < total) t = tile_of(at);
+      };
+      skip(first);
       auto fetch = [&] {
-        if (c.item >= total) return;
-        const int rows = X ? p.m : p.n, r0 = X ? c.t.row0 : c.t.f0;
-        const int in = min(rows - r0, X ? c.t.cols : kTileW) - lane;  // this lane's rows 32 q < in
-        const uint32_t *src = (X ? p.a_scales : p.b_scales + (size_t)c.t.g * p.words * p.n) + r0 + lane + (size_t)(2 * c.ks) * rows;
+        if (at.item >= total) return;
+        const int rows = X ? p.m : p.n, r0 = X ? t.row0 : t.f0;
+        const int in = min(rows - r0, X ? t.cols : kTileW) - lane;  // this lane's rows 32 q < in
+        const uint32_t *src = (X ? p.a_scales : p.b_scales + (size_t)t.g * p.words * p.n) + r0 + lane + (size_t)(2 * ks) * rows;
 #pragma unroll
         for (int w = 0; w < 2; ++w) {
-          const int lim = 2 * c.ks + w < p.words ? in : 0;
+          const int lim = 2 * ks + w < p.words ? in : 0;
 #pragma unroll
           for (int q = 0; q < Q; ++q) v[w][q] = 32 * q < lim ? __ldg(src + 32 * q) : 0u;
           src += rows;
         }
-        advance(c, kScaleWarps);
+        skip(kScaleWarps);
       };
       // this warp's stages
       const int mine = item0 < total ? ((total - 1 - item0) / step + 1) * (k_hi - k_lo) - first : 0;
@@ -449,8 +467,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     // ------------------------------------------------------------ epilogue
     const int q = warp & 3, half = (warp - 4) >> 2;  // TMEM lane quarter; which 32-column chunks
     int j = 0;
-    for (int item = item0; item < total; item += step, ++j) {
-      const Tile t = tile_at(item);
+    for (Walk w = start(); w.item < total; advance(w), ++j) {
+      const Tile t = tile_of(w);
       const int buf = j & 1;
       if (!mbar_wait(&acc_full[buf], (j >> 1) & 1, p.err, kMx4ErrWait)) break;
       tc_fence_after();
@@ -529,7 +547,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     // out = the parts of all ranks, added in rank order; rank r takes columns r, r + ranks, ...
     cluster_sync();
     if (item0 < total) {
-      const Tile t = tile_at(item0);
+      const Tile t = tile_of(start());
       const int fl = threadIdx.x & (kTileW - 1), f = t.f0 + fl;
       if (threadIdx.x < 2 * kTileW && f < p.n) {
         const float bias = p.bias ? bf16_to_f32(__ldg(p.bias + (size_t)t.g * p.n + f)) : 0.f;
