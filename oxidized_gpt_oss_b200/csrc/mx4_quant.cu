@@ -78,6 +78,28 @@ struct Raw {
   }
 };
 
+// Two f32 operations in one instruction (each rounded on its own).
+__device__ __forceinline__ uint64_t pair(float lo, float hi) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+  return r;
+}
+__device__ __forceinline__ float2 halves(uint64_t v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+
 // Eight values to four code bytes, element 0 in the lowest half byte.
 __device__ __forceinline__ uint32_t e2m1_pack8(const float (&v)[8]) {
   uint32_t r;
@@ -93,8 +115,13 @@ __device__ __forceinline__ uint32_t e2m1_pack8(const float (&v)[8]) {
 }
 __device__ __forceinline__ uint32_t pack_scaled(const float (&v)[8], float f) {
   float r[8];
+  const uint64_t f2 = pair(f, f);
 #pragma unroll
-  for (int i = 0; i < 8; ++i) r[i] = v[i] * f;
+  for (int i = 0; i < 8; i += 2) {
+    const float2 t = halves(mul2(pair(v[i], v[i + 1]), f2));
+    r[i] = t.x;
+    r[i + 1] = t.y;
+  }
   return e2m1_pack8(r);
 }
 
@@ -188,16 +215,27 @@ __device__ __forceinline__ uint32_t swiglu_quantize8_f64(const float (&gu)[16], 
 }
 __device__ __forceinline__ uint32_t swiglu_quantize8(const float (&gu)[16], float alpha, float limit, int rule, int *byte) {
   const float c = -alpha * 1.4426950408889634f;  // e^(-alpha g) = 2^(c g)
-  float h[8], sum = 0.f;
+  const uint64_t one = pair(1.f, 1.f), c2 = pair(c, c);
+  float h[8];
+  uint64_t sum2 = 0ull;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const float g = min_nan(gu[2 * i], limit), u = max_nan(min_nan(gu[2 * i + 1], limit), -limit);
-    float e, r;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(c * g));
-    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + e));
-    h[i] = g * r * (u + 1.0f);
-    sum += e;
+  for (int i = 0; i < 8; i += 2) {
+    const uint64_t g = pair(min_nan(gu[2 * i], limit), min_nan(gu[2 * i + 2], limit));
+    const uint64_t u = pair(max_nan(min_nan(gu[2 * i + 1], limit), -limit), max_nan(min_nan(gu[2 * i + 3], limit), -limit));
+    const float2 x = halves(mul2(c2, g));
+    float2 e, r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e.x) : "f"(x.x));
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e.y) : "f"(x.y));
+    const uint64_t e2 = pair(e.x, e.y);
+    const float2 d = halves(add2(one, e2));
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r.x) : "f"(d.x));
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r.y) : "f"(d.y));
+    const float2 v = halves(mul2(mul2(g, pair(r.x, r.y)), add2(u, one)));
+    h[i] = v.x;
+    h[i + 1] = v.y;
+    sum2 = add2(sum2, e2);
   }
+  const float sum = halves(sum2).x + halves(sum2).y;
   bool close = sum > 0x1p57f;  // some x beyond 40 (40 log2 e > 57)
   if (!(limit <= 0x1p18f)) {   // without a clamp that means something, every gate that is neither 0 nor ordinary
 #pragma unroll

@@ -79,7 +79,7 @@ _device_ctx: dict[int, abi.Context] = {}
 def device_context(x: torch.Tensor, ctx: abi.Context | None) -> abi.Context:
     """The given context, or a per-process one on x's device, bound to torch's
     current stream there."""
-    index = x.device.index
+    index = x.get_device()
     if ctx is None:
         ctx = _default_ctx if _default_ctx is not None and _default_ctx.device == index else _device_ctx.get(index)
         if ctx is None:
@@ -171,43 +171,43 @@ def tile_scales(scales: torch.Tensor, *, ctx: abi.Context | None = None) -> torc
     return out
 
 
-def _operand(blocks: torch.Tensor, scales: torch.Tensor, name: str, dim: int, device,
+def _operand(blocks: torch.Tensor, scales: torch.Tensor, name: str, dim: int, index: int,
              ctx: abi.Context | None) -> tuple[torch.Tensor, torch.Tensor]:
     """One operand's blocks and tiled scales, contiguous, checked against each other."""
     if blocks.dtype != torch.uint8 or scales.dtype != torch.uint8 or not blocks.is_cuda or \
-            blocks.device != device or scales.device != device:
+            blocks.get_device() != index or scales.get_device() != index:
         raise ValueError(f"{name}'s blocks and scales must be uint8 tensors on one CUDA device with the other operand")
-    if blocks.dim() != dim:
-        raise ValueError(f"{name}'s blocks must have {dim} dimensions, got {tuple(blocks.shape)}")
-    *lead, rows, half = blocks.shape
-    k = 2 * half
+    shape = blocks.shape
+    if len(shape) != dim:
+        raise ValueError(f"{name}'s blocks must have {dim} dimensions, got {tuple(shape)}")
+    lead, rows, k = shape[:-2], shape[-2], 2 * shape[-1]
     if k == 0 or k % 32:
         raise ValueError(f"k must be a positive multiple of 32, got {k}")
-    if scales.dim() == dim and tuple(scales.shape) == (*lead, rows, k // 32):
+    if scales.shape != (*lead, (k + 127) // 128, rows, 4):
+        if scales.shape != (*lead, rows, k // 32):
+            raise ValueError(f"{name}'s scales must be {(*lead, (k + 127) // 128, rows, 4)} (tiled) or "
+                             f"{(*lead, rows, k // 32)}, got {tuple(scales.shape)}")
         scales = tile_scales(scales, ctx=ctx)
-    elif tuple(scales.shape) != (*lead, (k + 127) // 128, rows, 4):
-        raise ValueError(f"{name}'s scales must be {(*lead, (k + 127) // 128, rows, 4)} (tiled) or {(*lead, rows, k // 32)}, "
-                         f"got {tuple(scales.shape)}")
     return blocks.contiguous(), scales.contiguous()
 
 
-def _output(out: torch.Tensor | None, out_dtype: torch.dtype, m: int, n: int, device) -> tuple[torch.Tensor, int, int]:
-    """The output tensor, its type's code and its row pitch."""
+def _output(out: torch.Tensor | None, out_dtype: torch.dtype, m: int, n: int, a: torch.Tensor) -> tuple[torch.Tensor, int, int]:
+    """The output tensor (a new one on a's device), its type's code and its row pitch."""
     if out is None:
         if out_dtype not in (torch.float32, torch.bfloat16):
             raise ValueError(f"out_dtype must be float32 or bfloat16, got {out_dtype}")
-        out = torch.empty(m, n, dtype=out_dtype, device=device)
-    elif tuple(out.shape) != (m, n) or out.dtype not in (torch.float32, torch.bfloat16) or out.device != device or \
+        return a.new_empty((m, n), dtype=out_dtype), _DTYPES[out_dtype], n
+    if out.shape != (m, n) or out.dtype not in (torch.float32, torch.bfloat16) or out.device != a.device or \
             (n > 1 and out.stride(1) != 1) or (m > 1 and out.stride(0) < n):
-        raise ValueError(f"out must be a float32 or bfloat16 [{m}, {n}] on {device} with contiguous rows")
+        raise ValueError(f"out must be a float32 or bfloat16 [{m}, {n}] on {a.device} with contiguous rows")
     return out, _DTYPES[out.dtype], out.stride(0) if m > 1 else n
 
 
-def _bias(bias: torch.Tensor | None, shape: tuple, device) -> torch.Tensor | None:
+def _bias(bias: torch.Tensor | None, shape: tuple, index: int) -> torch.Tensor | None:
     if bias is None:
         return None
-    if bias.dtype != torch.bfloat16 or tuple(bias.shape) != shape or bias.device != device:
-        raise ValueError(f"bias must be bfloat16 {shape} on {device}, got {bias.dtype} {tuple(bias.shape)}")
+    if bias.dtype != torch.bfloat16 or bias.shape != shape or bias.get_device() != index:
+        raise ValueError(f"bias must be bfloat16 {shape} on cuda:{index}, got {bias.dtype} {tuple(bias.shape)}")
     return bias.contiguous()
 
 
@@ -217,14 +217,15 @@ def mxfp4_matmul(a_blocks: torch.Tensor, a_scales: torch.Tensor, b_blocks: torch
     """a [m, k] times b [n, k] transposed, plus ``bias`` [n] (bfloat16), both
     operands MXFP4 (blocks [rows, k / 2], scales tiled [ceil(k / 128), rows, 4] or
     [rows, k / 32]); f32 sums, returned as ``out_dtype`` (float32 or bfloat16)."""
-    device = a_blocks.device
-    a_blocks, a_scales = _operand(a_blocks, a_scales, "a", 2, device, ctx)
-    b_blocks, b_scales = _operand(b_blocks, b_scales, "b", 2, device, ctx)
-    m, n, k = a_blocks.shape[0], b_blocks.shape[0], 2 * a_blocks.shape[1]
+    index = a_blocks.get_device()
+    a_blocks, a_scales = _operand(a_blocks, a_scales, "a", 2, index, ctx)
+    b_blocks, b_scales = _operand(b_blocks, b_scales, "b", 2, index, ctx)
+    m, half = a_blocks.shape
+    n, k = b_blocks.shape[0], 2 * half
     if 2 * b_blocks.shape[1] != k:
         raise ValueError(f"a has rows of {k} elements, b of {2 * b_blocks.shape[1]}")
-    out, code, ldo = _output(out, out_dtype, m, n, device)
-    bias = _bias(bias, (n,), device)
+    out, code, ldo = _output(out, out_dtype, m, n, a_blocks)
+    bias = _bias(bias, (n,), index)
     c = device_context(a_blocks, ctx)
     check_status(c.lib.oxg_mxfp4_matmul(c.handle, a_blocks.data_ptr(), a_scales.data_ptr(), m, b_blocks.data_ptr(),
                                         b_scales.data_ptr(), n, k, None if bias is None else bias.data_ptr(),
@@ -242,18 +243,19 @@ def mxfp4_grouped_matmul(a_blocks: torch.Tensor, a_scales: torch.Tensor, counts:
     them). bias [groups, n] bfloat16. Rows past the last group keep what ``out``
     held (nothing in particular in a new one). Counts that are negative or add
     up to more than m are reported by the context's next ``sync``."""
-    device = a_blocks.device
-    a_blocks, a_scales = _operand(a_blocks, a_scales, "a", 2, device, ctx)
-    b_blocks, b_scales = _operand(b_blocks, b_scales, "b", 3, device, ctx)
-    m, k = a_blocks.shape[0], 2 * a_blocks.shape[1]
+    index = a_blocks.get_device()
+    a_blocks, a_scales = _operand(a_blocks, a_scales, "a", 2, index, ctx)
+    b_blocks, b_scales = _operand(b_blocks, b_scales, "b", 3, index, ctx)
+    m, half = a_blocks.shape
+    k = 2 * half
     groups, n = b_blocks.shape[:2]
     if 2 * b_blocks.shape[2] != k:
         raise ValueError(f"a has rows of {k} elements, b of {2 * b_blocks.shape[2]}")
-    if counts.dtype != torch.int32 or tuple(counts.shape) != (groups,) or counts.device != device:
-        raise ValueError(f"counts must be int32 [{groups}] on {device}, got {counts.dtype} {tuple(counts.shape)}")
+    if counts.dtype != torch.int32 or counts.shape != (groups,) or counts.get_device() != index:
+        raise ValueError(f"counts must be int32 [{groups}] on cuda:{index}, got {counts.dtype} {tuple(counts.shape)}")
     counts = counts.contiguous()
-    out, code, ldo = _output(out, out_dtype, m, n, device)
-    bias = _bias(bias, (groups, n), device)
+    out, code, ldo = _output(out, out_dtype, m, n, a_blocks)
+    bias = _bias(bias, (groups, n), index)
     c = device_context(a_blocks, ctx)
     check_status(c.lib.oxg_mxfp4_grouped_matmul(c.handle, a_blocks.data_ptr(), a_scales.data_ptr(), m, counts.data_ptr(),
                                                 groups, b_blocks.data_ptr(), b_scales.data_ptr(), n, k,
