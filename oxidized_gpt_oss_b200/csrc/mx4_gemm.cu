@@ -14,10 +14,10 @@
 // l + 96 (each load coalesced) and stores them as the 16 bytes that the tensor core's scale atom (128 rows x
 // 4 blocks, row r at 16 (r % 32) + 4 (r / 32)) has for it.
 //
-// Two kernels share this code. For many rows, pairs of CTAs (cta_group::2) work on 256 weight rows x up to 224
+// Three kernels share this code. For many rows, pairs of CTAs (cta_group::2) work on 256 weight rows x up to 224
 // activation rows, so that each SM fetches and reads half of the activation codes. For few rows, a CTA
 // works on 128 weight rows x up to 64 activation rows, with more stages of weight codes in flight, and where
-// there are fewer tiles than SMs, a cluster splits a tile's K and adds the parts through distributed shared
+// there are far fewer tiles than SMs, a cluster splits a tile's K and adds the parts through distributed shared
 // memory in rank order (so a result does not depend on timing).
 //
 // CTAs walk their tiles with the weight tile fastest: CTAs side by side share activation rows, and a group's
@@ -46,6 +46,7 @@ constexpr int kStageK = 256;          // elements of K per stage: 128 bytes of c
 constexpr int kEpiWarps = 8;           // two for each quarter of the TMEM lanes, taking 32 columns in turn
 constexpr int kScaleWarps = 4;         // for each operand; a stage belongs to one of them
 constexpr int kThreads = 32 * (2 + kEpiWarps + 2 * kScaleWarps);
+constexpr int kMaxRanks = 8;           // CTAs that split a tile's K (the portable cluster size)
 constexpr int kWBytes = kTileW * 128;  // a stage's weight codes
 
 // PAIR: two CTAs per tile. NMAX: most activation rows per tile. SPLIT: a cluster per tile, K split.
@@ -118,9 +119,12 @@ __device__ __forceinline__ void umma_commit_both(uint64_t *bar) {
       "h"((uint16_t)3)
       : "memory");
 }
-__device__ __forceinline__ float ld_cluster_f32(uint32_t addr_cl) {
-  float v;
-  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr_cl) : "memory");
+__device__ __forceinline__ float4 ld_cluster_f32x4(uint32_t addr_cl) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+               : "r"(addr_cl)
+               : "memory");
   return v;
 }
 __device__ __forceinline__ uint32_t pack_bf16x2(float lo, float hi) {
@@ -544,21 +548,38 @@ __global__ void __launch_bounds__(kThreads, 1)
   __syncthreads();
   tc_fence_after();
   if (SPLIT) {
-    // out = the parts of all ranks, added in rank order; rank r takes columns r, r + ranks, ...
+    // out = the parts of all ranks, added in rank order; rank r takes columns r, r + ranks, ..., a warp one of
+    // them at a time, four features a lane, the ranks' loads all on their way before the first is added
     cluster_sync();
     if (item0 < total) {
       const Tile t = tile_of(start());
-      const int fl = threadIdx.x & (kTileW - 1), f = t.f0 + fl;
-      if (threadIdx.x < 2 * kTileW && f < p.n) {
-        const float bias = p.bias ? bf16_to_f32(__ldg(p.bias + (size_t)t.g * p.n + f)) : 0.f;
-        for (int c = (int)rank + (int)(threadIdx.x / kTileW) * (int)n_ranks; c < t.rows; c += 2 * (int)n_ranks) {
-          const uint32_t part = smem_addr(stages) + (uint32_t)(c * kTileW + fl) * 4;
-          float sum = 0.f;
-          for (uint32_t r = 0; r < n_ranks; ++r) sum += ld_cluster_f32(mapa_shared(part, r));
-          sum += bias;
-          const size_t o = (size_t)(t.row0 + c) * p.ldo + f;
-          if (p.out_bf16) static_cast<uint16_t *>(p.out)[o] = (uint16_t)pack_bf16x2(sum, 0.f);
-          else static_cast<float *>(p.out)[o] = sum;
+      const int f = t.f0 + 4 * lane;
+      float bias[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        bias[i] = p.bias && f + i < p.n ? bf16_to_f32(__ldg(p.bias + (size_t)t.g * p.n + f + i)) : 0.f;
+      for (int c = (int)rank + warp * (int)n_ranks; c < t.rows; c += kThreads / 32 * (int)n_ranks) {
+        const uint32_t part = smem_addr(stages) + (uint32_t)(c * kTileW + 4 * lane) * 4;
+        float4 v[kMaxRanks];
+#pragma unroll
+        for (int r = 0; r < kMaxRanks; ++r)
+          if (r < (int)n_ranks) v[r] = ld_cluster_f32x4(mapa_shared(part, r));
+        float4 sum = v[0];
+#pragma unroll
+        for (int r = 1; r < kMaxRanks; ++r)
+          if (r < (int)n_ranks) {
+            sum.x += v[r].x;
+            sum.y += v[r].y;
+            sum.z += v[r].z;
+            sum.w += v[r].w;
+          }
+        const float y[4] = {sum.x + bias[0], sum.y + bias[1], sum.z + bias[2], sum.w + bias[3]};
+        const size_t o = (size_t)(t.row0 + c) * p.ldo + f;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          if (f + i >= p.n) break;
+          if (p.out_bf16) static_cast<uint16_t *>(p.out)[o + i] = (uint16_t)pack_bf16x2(y[i], 0.f);
+          else static_cast<float *>(p.out)[o + i] = y[i];
         }
       }
     }
@@ -656,6 +677,31 @@ using Pair = Cfg<true, 224, 6, false>;
 using Few = Cfg<false, 64, 8, false>;
 using FewSplit = Cfg<false, 64, 8, true>;
 
+// Clusters of `ranks` CTAs that the GPU holds side by side (its processing clusters are not multiples of it).
+int clusters_at_once(int ranks, int n_sms) {
+  static std::atomic<int> known[kMaxRanks + 1];
+  int n = known[ranks].load(std::memory_order_relaxed);
+  if (n) return n;
+  auto kern = mx4_gemm_kernel<FewSplit>;
+  cudaLaunchConfig_t cfg{};
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = (unsigned)ranks;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.blockDim = dim3(kThreads);
+  cfg.gridDim = dim3((unsigned)(n_sms / ranks * ranks));
+  cfg.dynamicSmemBytes = FewSplit::SMEM;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, FewSplit::SMEM) != cudaSuccess ||
+      cudaOccupancyMaxActiveClusters(&n, kern, &cfg) != cudaSuccess || n < 1) {
+    cudaGetLastError();
+    n = 1;
+  }
+  known[ranks].store(n, std::memory_order_relaxed);
+  return n;
+}
+
 }  // namespace
 
 cudaError_t launch_mx4_gemm(const Mx4GemmArgs &a, int n_sms, cudaStream_t stream) {
@@ -676,10 +722,26 @@ cudaError_t launch_mx4_gemm(const Mx4GemmArgs &a, int n_sms, cudaStream_t stream
   p.out_bf16 = a.out_bf16;
   p.pair_stores = a.n % 2 == 0 && (a.ldo % 2 == 0 || a.m == 1) && (uintptr_t)a.out % 4 == 0;
   p.err = a.err;
-  if ((long long)a.m > 64ll * a.groups) return launch_cfg<Pair>(a, p, n_sms, 1, stream);
-  const long long tiles = ((long long)a.n + kTileW - 1) / kTileW * std::min(a.groups, a.m);
-  int ranks = 1;  // CTAs per tile: a power of two that leaves each at least two stages
-  while (ranks < 8 && 2 * ranks * tiles <= n_sms && 4 * ranks <= p.k_steps) ranks *= 2;
+  // Which kernel: estimates in ns from launches back to back on a B200 (k 512 .. 8192, n 640 .. 20480, m 1 .. 1024,
+  // codes in L2). A launch costs 4100 with single CTAs and 5000 with pairs; a stage 265 in a CTA with up to 64
+  // rows, 270 in a pair with up to 128 and 300 above; adding up a split 1300 + 17 a column. For instance 448 x 2880
+  // x 2880 takes 9.0 us in pairs and 10.9 in CTAs (two rounds of tiles), 256 x 2880 x 2880 8.4 and 7.6; 64 x 2880 x
+  // 8192 12.6 unsplit and 8.8 over 4 CTAs, 64 x 2880 x 2880 7.3 and 7.6. Bound by HBM they are alike (64 x 201088 x
+  // 2880: 55.6 and 56.9). Groups count as if they had even shares of the rows.
+  const long long held = std::min(a.groups, a.m), rows = (a.m + held - 1) / held;
+  auto tiles = [&](int w, int x) { return (a.n + w - 1ll) / w * held * ((rows + x - 1) / x); };
+  const long long few_tiles = tiles(kTileW, Few::NMAX), pair_tiles = tiles(2 * kTileW, Pair::NMAX);
+  const long long pair_ns = 5000 + (pair_tiles + n_sms / 2 - 1) / (n_sms / 2) * p.k_steps * (rows > 128 ? 300 : 270);
+  long long few_ns = 4100 + (few_tiles + n_sms - 1) / n_sms * p.k_steps * 265;
+  int ranks = 1;
+  for (int r = 2; r <= kMaxRanks && 2 * r <= p.k_steps && r * few_tiles <= n_sms; ++r) {
+    const long long ns = 4100 + (p.k_steps + r - 1) / r * 265 + 1300 + 17 * std::min<long long>(rows, Few::NMAX);
+    if (ns < few_ns && few_tiles <= clusters_at_once(r, n_sms)) {
+      few_ns = ns;
+      ranks = r;
+    }
+  }
+  if (pair_ns < few_ns) return launch_cfg<Pair>(a, p, n_sms, 1, stream);
   if (ranks > 1) return launch_cfg<FewSplit>(a, p, n_sms, ranks, stream);
   return launch_cfg<Few>(a, p, n_sms, 1, stream);
 }

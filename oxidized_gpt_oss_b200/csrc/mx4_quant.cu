@@ -19,7 +19,7 @@
 namespace oxg {
 namespace {
 
-constexpr int kThreads = 256;
+constexpr int kThreads = 128;  // SwiGLU prompt from bf16: 85 us, against 95 with 256 threads, 107 with 512 and 100 with 64
 
 template <int T>
 struct Elem;
@@ -416,7 +416,7 @@ cudaError_t launch_mx4_tile_scales(const uint8_t *src, size_t groups, size_t row
   const uint32_t kb = (uint32_t)(cols / 32), words = (kb + 3) / 4;
   const size_t n_words = groups * rows * words;
   if (n_words == 0) return cudaSuccess;
-  const size_t want = (n_words + kThreads - 1) / kThreads, cap = (size_t)n_sms * 16;
+  const size_t want = (n_words + kThreads - 1) / kThreads, cap = (size_t)n_sms * 32;
   return launch_dependent(mx4_tile_scales_kernel, (unsigned)(want < cap ? want : cap), stream, src, n_words, rows, kb, words,
                           reinterpret_cast<uint32_t *>(dst));
 }

@@ -246,7 +246,8 @@ def _bias(rng, *shape):
 
 SHAPES = [(1, 1, 32), (1, 5, 32), (2, 128, 64), (16, 129, 96), (17, 64, 128), (31, 300, 160), (33, 127, 256), (64, 1000, 288),
           (128, 130, 512), (129, 256, 544), (224, 33, 1024), (225, 77, 1056), (300, 257, 2880), (449, 128, 64), (1000, 640, 2880),
-          (8, 5120, 2880), (1, 2880, 4096), (50, 96, 8192), (700, 1, 320), (1037, 2881, 224)]
+          (8, 5120, 2880), (1, 2880, 4096), (50, 96, 8192), (700, 1, 320), (1037, 2881, 224),
+          (40, 38500, 544), (3, 19300, 2400), (100, 60, 8192), (2000, 1300, 1184)]
 
 
 @pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
@@ -348,6 +349,26 @@ def test_grouped_matmul_at_gpt_oss_widths(cuda_ctx):
     for g, cnt in enumerate(counts):
         _check(got[r: r + cnt], av[r: r + cnt], ref.values(bb[g], bsc[g]), None, "bfloat16")
         r += cnt
+
+
+def test_grouped_matmul_of_few_rows_and_many_tiles(cuda_ctx):
+    """More tiles than SMs with a handful of rows each: a CTA goes through several tiles of different groups."""
+    torch, mxfp4, _ = _torch()
+    rng = np.random.default_rng(14)
+    counts = np.array([3, 0, 17, 1, 65, 0, 0, 2, 8, 30])
+    m, n, k = int(counts.sum()) + 5, 5764, 2400
+    (ab, asc), (bb, bsc) = _operand(rng, m, k), _operand(rng, len(counts), n, k, around=122)
+    bias, bias64 = _bias(rng, len(counts), n)
+    a, at, b, bt, c = _cuda(ab, ref.tile(asc, k), bb, ref.tile(bsc, k), counts.astype(np.int32))
+    for dtype in (torch.float32, torch.bfloat16):
+        out = torch.full((m, n), 55.0, device="cuda", dtype=dtype)
+        mxfp4.mxfp4_grouped_matmul(a, at, c, b, bt, bias=bias, out=out)
+        cuda_ctx.sync()
+        av, r = ref.values(ab, asc), 0
+        for g, cnt in enumerate(counts):
+            _check(out[r: r + cnt], av[r: r + cnt], ref.values(bb[g], bsc[g]), bias64[g], str(dtype)[6:])
+            r += cnt
+        assert (out[r:] == 55.0).all()
 
 
 @pytest.mark.parametrize("counts", [[20, 30], [-1, 20], [2 ** 31 - 1, 2 ** 31 - 1], [41, 0]])
