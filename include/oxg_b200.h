@@ -115,7 +115,8 @@ OXG_API int oxg_swiglu(oxg_ctx *ctx, const float *gate_dev, const float *up_dev,
  *                     written as 0 here). A weight is laid out once with
  *                     oxg_mxfp4_tile_scales; the quantisers write either.
  * These calls keep nothing between them and use no workspace: calls on several
- * streams, or replays of several captured graphs, do not disturb one another. */
+ * streams, or replays of several captured graphs, do not disturb one another.
+ * The same call gives the same bits every time. */
 enum { OXG_DTYPE_F32 = 0, OXG_DTYPE_BF16 = 1, OXG_DTYPE_F16 = 2 };
 /* A block with largest magnitude t in [2^e, 2^(e+1)) gets the scale 2^(e-2)
  * (FLOOR: what then lies above E2M1's largest value 6 becomes 6), or twice
@@ -462,7 +463,8 @@ OXG_API int oxg_model_release(oxg_ctx *ctx);
 OXG_API int oxg_profile_enable(oxg_ctx *ctx, int on);
 /* Total device time (ms) and launch count of kernel `name` since the last
  * reset (names: router_topk, permute, moe_mlp1_decode, moe_mlp2_decode,
- * combine, dequant_mxfp4, swiglu). Waits for the context's stream. */
+ * combine, dequant_mxfp4, swiglu, quantize_mxfp4, swiglu_quantize_mxfp4,
+ * mxfp4_tile_scales, mxfp4_matmul, mxfp4_grouped_matmul). Waits for the context's stream. */
 OXG_API int oxg_profile_read(oxg_ctx *ctx, const char *name, double *total_ms, int *launches);
 OXG_API int oxg_profile_reset(oxg_ctx *ctx);
 /* Number of kernels this context has launched since it was created. */

@@ -83,8 +83,12 @@ int quantize(oxg_ctx *ctx, oxg::Mx4QuantArgs &a, int dtype, bool swiglu) {
   });
 }
 
+constexpr int kMost = 0x7FFFFE00;  // 32-bit numbers with room for a tile
+
 int product(oxg_ctx *ctx, oxg::Mx4GemmArgs &a, int out_dtype) {
   if (a.m < 0 || a.n < 0) return fail(ctx, OXG_ERR_SHAPE, "m and n must not be negative, got %d and %d", a.m, a.n);
+  if (a.m > kMost || a.n > kMost || a.k > kMost)
+    return fail(ctx, OXG_ERR_SHAPE, "m, n and k must be at most %d, got %d, %d and %d", kMost, a.m, a.n, a.k);
   if (a.k <= 0 || a.k % 32) return fail(ctx, OXG_ERR_SHAPE, "k must be a positive multiple of 32, got %d", a.k);
   if (out_dtype != OXG_DTYPE_F32 && out_dtype != OXG_DTYPE_BF16)
     return fail(ctx, OXG_ERR_INVALID_ARG, "the output must be f32 or bf16, got element type %d", out_dtype);

@@ -633,7 +633,7 @@ cudaError_t launch_cfg(const Mx4GemmArgs &a, Params &p, int n_sms, int ranks, cu
   const long long x_tiles = a.counts ? (long long)a.m / C::NMAX + std::min(a.groups, a.m) : ((long long)a.m + C::NMAX - 1) / C::NMAX;
   // one box where all tiles are alike; else two at most (16-row steps would be seven copies a stage)
   if (a.counts) p.box = C::NMAX / C::CTAS / 2;
-  else p.box = round_cols<C>((a.m + (int)x_tiles - 1) / (int)x_tiles) / C::CTAS;
+  else p.box = round_cols<C>((int)((a.m + x_tiles - 1) / x_tiles)) / C::CTAS;
   CUtensorMap tm_x, tm_w;
   cudaError_t st;
   if ((st = code_map(&tm_x, a.a, 2, a.k, a.m, 1, p.box))) return st;
@@ -730,12 +730,13 @@ cudaError_t launch_mx4_gemm(const Mx4GemmArgs &a, int n_sms, cudaStream_t stream
   // 2880: 55.6 and 56.9). Groups count as if they had even shares of the rows.
   const long long held = std::min(a.groups, a.m), rows = (a.m + held - 1) / held;
   auto tiles = [&](int w, int x) { return (a.n + w - 1ll) / w * held * ((rows + x - 1) / x); };
+  auto rounds = [](long long tiles, int at_once) { return (double)((tiles + at_once - 1) / at_once); };
   const long long few_tiles = tiles(kTileW, Few::NMAX), pair_tiles = tiles(2 * kTileW, Pair::NMAX);
-  const long long pair_ns = 5000 + (pair_tiles + n_sms / 2 - 1) / (n_sms / 2) * p.k_steps * (rows > 128 ? 300 : 270);
-  long long few_ns = 4100 + (few_tiles + n_sms - 1) / n_sms * p.k_steps * 265;
+  const double pair_ns = 5000 + rounds(pair_tiles, n_sms / 2) * p.k_steps * (rows > 128 ? 300 : 270);
+  double few_ns = 4100 + rounds(few_tiles, n_sms) * p.k_steps * 265;
   int ranks = 1;
   for (int r = 2; r <= kMaxRanks && 2 * r <= p.k_steps && r * few_tiles <= n_sms; ++r) {
-    const long long ns = 4100 + (p.k_steps + r - 1) / r * 265 + 1300 + 17 * std::min<long long>(rows, Few::NMAX);
+    const double ns = 4100 + (p.k_steps + r - 1) / r * 265. + 1300 + 17. * std::min<long long>(rows, Few::NMAX);
     if (ns < few_ns && few_tiles <= clusters_at_once(r, n_sms)) {
       few_ns = ns;
       ranks = r;

@@ -14,22 +14,25 @@ The way back and what 4-bit operands are for (no counterpart in the reference):
 their own (experts). The products read scales in the tiled layout
 ``[ceil(k / 128), rows, 4]``, which the quantisers write with ``tiled=True`` and
 ``tile_scales`` makes of a checkpoint's ``[rows, k / 32]``; given the latter,
-they convert it first, on every call.
+they convert it first, on every call. The first call on a device creates its
+context, which allocates: make it before a stream capture.
 """
 from __future__ import annotations
+
+import threading
 
 import torch
 
 from . import abi
 
 _default_ctx = None
+# the raw stream handle where this torch has it: the Stream object costs 3 us a call
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 
 
 def _bind(ctx: abi.Context) -> abi.Context:
     """Puts the context on torch's current stream of its device."""
-    # the raw handle where this torch has it: the Stream object costs 3 us a call
-    raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
-    stream = raw(ctx.device) if raw is not None else torch.cuda.current_stream(ctx.device).cuda_stream
+    stream = _raw_stream(ctx.device) if _raw_stream is not None else torch.cuda.current_stream(ctx.device).cuda_stream
     abi.check(ctx.lib.oxg_ctx_set_stream(ctx.handle, stream), ctx.handle)
     return ctx
 
@@ -74,16 +77,27 @@ def dequantize_mxfp4(blocks: torch.Tensor, scales: torch.Tensor, rows: int, cols
 _DTYPES = {torch.float32: abi.OXG_DTYPE_F32, torch.bfloat16: abi.OXG_DTYPE_BF16, torch.float16: abi.OXG_DTYPE_F16}
 _RULES = {"floor": abi.OXG_MX_FLOOR, "noclip": abi.OXG_MX_NOCLIP}
 _device_ctx: dict[int, abi.Context] = {}
+_main_thread = threading.main_thread().ident
+_other_threads = threading.local()
+_MOST = 0x7FFFFE00  # rows, columns and k of a product: 32-bit numbers with room for a tile
 
 
 def device_context(x: torch.Tensor, ctx: abi.Context | None) -> abi.Context:
-    """The given context, or a per-process one on x's device, bound to torch's
-    current stream there."""
+    """The given context, or the calling thread's own on x's device (the main
+    thread's is the process's default one), bound to torch's current stream there."""
     index = x.get_device()
     if ctx is None:
-        ctx = _default_ctx if _default_ctx is not None and _default_ctx.device == index else _device_ctx.get(index)
-        if ctx is None:
-            ctx = _device_ctx[index] = abi.Context(index)
+        if threading.get_ident() != _main_thread:
+            own = _other_threads.__dict__
+            ctx = own.get(index)
+            if ctx is None:
+                ctx = own[index] = abi.Context(index)
+        elif _default_ctx is not None and _default_ctx.device == index:
+            ctx = _default_ctx
+        else:
+            ctx = _device_ctx.get(index)
+            if ctx is None:
+                ctx = _device_ctx[index] = abi.Context(index)
     elif ctx.device != index:
         raise ValueError(f"the context is on cuda:{ctx.device}, the input on {x.device}")
     return _bind(ctx)
@@ -183,6 +197,8 @@ def _operand(blocks: torch.Tensor, scales: torch.Tensor, name: str, dim: int, in
     lead, rows, k = shape[:-2], shape[-2], 2 * shape[-1]
     if k == 0 or k % 32:
         raise ValueError(f"k must be a positive multiple of 32, got {k}")
+    if rows > _MOST or k > _MOST:
+        raise ValueError(f"{name} is too large: {rows} rows of {k} elements")
     if scales.shape != (*lead, (k + 127) // 128, rows, 4):
         if scales.shape != (*lead, rows, k // 32):
             raise ValueError(f"{name}'s scales must be {(*lead, (k + 127) // 128, rows, 4)} (tiled) or "

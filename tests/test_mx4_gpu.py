@@ -417,6 +417,8 @@ def test_product_refusals(cuda_ctx):
     q = o.data_ptr()
     for status, args in ((abi.OXG_ERR_SHAPE, (p, sp, -1, p, sp, 4, 64, None, q, 0, 4)), (abi.OXG_ERR_SHAPE, (p, sp, 4, p, sp, 4, 48, None, q, 0, 4)),
                          (abi.OXG_ERR_SHAPE, (p, sp, 4, p, sp, 4, 0, None, q, 0, 4)), (abi.OXG_ERR_SHAPE, (p, sp, 4, p, sp, 4, 64, None, q, 0, 3)),
+                         (abi.OXG_ERR_SHAPE, (p, sp, 2 ** 31 - 1, p, sp, 4, 64, None, q, 0, 4)),
+                         (abi.OXG_ERR_SHAPE, (p, sp, 4, p, sp, 2 ** 31 - 256, 64, None, q, 0, 2 ** 31)),
                          (abi.OXG_ERR_INVALID_ARG, (p, sp, 4, p, sp, 4, 64, None, q, 2, 4)),
                          (abi.OXG_ERR_INVALID_ARG, (p + 8, sp, 2, p, sp, 4, 32, None, q, 0, 4)),
                          (abi.OXG_ERR_INVALID_ARG, (p, sp + 1, 2, p, sp, 4, 32, None, q, 0, 4)),
@@ -479,6 +481,78 @@ def test_graphs_and_streams(cuda_ctx):
     torch.cuda.synchronize()
     for w, o in zip(want, outs):
         assert torch.equal(w, o)
+    cuda_ctx.sync()
+
+
+def test_threads_on_streams_of_their_own(cuda_ctx):
+    """Two host threads without a context of their own, each on its own stream, calling at once."""
+    import threading
+    torch, mxfp4, _ = _torch()
+    w = mxfp4.quantize_mxfp4(torch.randn(2000, 1024, device="cuda"), tiled=True)
+    xs = [torch.randn(m, 1024, device="cuda") for m in (40, 900)]
+    want = [mxfp4.mxfp4_matmul(*mxfp4.quantize_mxfp4(x, tiled=True), *w) for x in xs]
+    torch.cuda.synchronize()
+    bad, gate = [], threading.Barrier(2)
+
+    def work(x, y):
+        st = torch.cuda.Stream()
+        gate.wait()
+        with torch.cuda.stream(st):
+            for _ in range(100):
+                got = mxfp4.mxfp4_matmul(*mxfp4.quantize_mxfp4(x, tiled=True), *w)
+                st.synchronize()
+                if not torch.equal(got, y):
+                    bad.append(x.shape)
+        mxfp4.device_context(x, None).sync()
+
+    threads = [threading.Thread(target=work, args=a) for a in zip(xs, want)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not bad
+
+
+FIRST_IN_CAPTURE = """
+import torch
+from oxidized_gpt_oss_b200 import abi, mxfp4
+torch.cuda.set_device(0)
+mxfp4.context(None)
+x, w = torch.randn(70, 512, device="cuda"), torch.randn(300, 512, device="cuda")
+one = torch.randn(1, 4096, device="cuda"), torch.randn(300, 4096, device="cuda")
+torch.cuda.synchronize()
+g = torch.cuda.CUDAGraph()
+def work():
+    return [mxfp4.mxfp4_matmul(*mxfp4.quantize_mxfp4(a, tiled=True), *mxfp4.quantize_mxfp4(b, tiled=True)) for a, b in ((x, w), one)]
+with torch.cuda.graph(g):
+    out = work()
+g.replay()
+torch.cuda.synchronize()
+for a, b in zip(out, work()):
+    assert torch.equal(a, b)
+print("replayed")
+"""
+
+
+def test_first_calls_in_a_capture():
+    """A process whose first calls, once it has a context, are captured."""
+    import os
+    import subprocess
+    import sys
+    r = subprocess.run([sys.executable, "-c", FIRST_IN_CAPTURE], cwd=os.path.dirname(os.path.dirname(os.path.abspath(__file__))),
+                       capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "replayed" in r.stdout, r.stderr[-2000:]
+
+
+def test_empty_operands(cuda_ctx):
+    torch, mxfp4, ffn = _torch()
+    none, w = mxfp4.quantize_mxfp4(torch.empty(0, 64, device="cuda"), tiled=True), mxfp4.quantize_mxfp4(torch.randn(8, 64, device="cuda"), tiled=True)
+    assert mxfp4.mxfp4_matmul(*none, *w).shape == (0, 8)
+    assert mxfp4.mxfp4_matmul(*w, *none).shape == (8, 0)
+    b, s = mxfp4.quantize_mxfp4(torch.empty(0, 5, 64, device="cuda"))
+    out = torch.full((8, 5), 3.0, device="cuda")
+    assert (mxfp4.mxfp4_grouped_matmul(*w, torch.empty(0, dtype=torch.int32, device="cuda"), b, s, out=out) == 3).all()
+    assert ffn.swiglu_quantize_mxfp4(torch.empty(3, 0, device="cuda"))[0].shape == (3, 0)
     cuda_ctx.sync()
 
 
