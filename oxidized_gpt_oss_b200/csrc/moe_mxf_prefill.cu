@@ -96,14 +96,6 @@ __device__ __forceinline__ void umma_mxf_pair(uint32_t d_tmem, uint64_t a_desc, 
       "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate), "r"(sfa_tmem), "r"(sfb_tmem)
       : "memory");
 }
-__device__ __forceinline__ void tma_load_3d_pair(void *smem_dst, const void *tmap, uint32_t bar_cl, int c0, int c1,
-                                                 int c2) {
-  asm volatile(
-      "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes"
-      " [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(smem_addr(smem_dst)),
-      "l"(tmap), "r"(bar_cl), "r"(c0), "r"(c1), "r"(c2)
-      : "memory");
-}
 // Instruction descriptor: A = E4M3 activations, B = E2M1 weights.
 __host__ __device__ constexpr uint32_t idesc_e4m3_e2m1(int m, int n, int a_sf, int b_sf) {
   return ((uint32_t)b_sf << 4) | (0u << 7) | (5u << 10) | ((uint32_t)(n >> 3) << 17) | (1u << 23) |

@@ -20,6 +20,18 @@
 // there are far fewer tiles than SMs, a cluster splits a tile's K and adds the parts through distributed shared
 // memory in rank order (so a result does not depend on timing).
 //
+// What bounds it, and measured figures (B200; device time back to back):
+//   many rows: per stage and SM the tensor cores need 449 cycles (256 x 224 x 256 in a pair), the codes and scales
+//   come in at 34 KB (528 cycles at 64 bytes a cycle), and shared memory is written and read with some 60 KB;
+//   532 cycles measured. 8192^3: 182 us, 6.0 PFLOP/s (67 % of the kind::mxf4 rate) in bursts; for seconds on end
+//   the power cap takes the clock from 1965 to about 1455 MHz. 8192 x 5120 x 2880: 53 us, 4.6 PFLOP/s (12 stages
+//   a tile, and the ends of the launch). 32768 rows over 32 groups x 5760 x 2880: 262-278 us, 4.1 PFLOP/s.
+//   few rows: HBM. 64 x 201088 x 2880: 57-62 us, 5.8-6.3 TB/s; 32 rows over 27 of 32 groups x 5760 x 2880: 44 us,
+//   5.4 TB/s, of which about 4 us are the launch, the first stage's latency and the last epilogue.
+// Tried and left out: asking L2 for the next tile's codes ahead of TMA (decode 74 us instead of 44), L2 promotion
+// of 128 bytes or none (equal), tiles of 448 activation rows in both accumulators (a third less L2 traffic, but
+// nothing to compute while an epilogue of 2600 cycles runs, and coarser rounds of tiles).
+//
 // CTAs walk their tiles with the weight tile fastest: CTAs side by side share activation rows, and a group's
 // weights stay in L2. Warps: 0 TMA (codes, 128-byte swizzle), 1 MMA, 2-3 and 12-17 scales (four for the weights'
 // words and four for the activations', a stage each in turn; the words of a warp's next stage are on their way
@@ -104,20 +116,11 @@ __device__ __forceinline__ void umma_mxf4_pair(uint32_t d_tmem, uint64_t a_desc,
       "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate), "r"(sfa_tmem), "r"(sfb_tmem)
       : "memory");
 }
-__device__ __forceinline__ void tma_load_3d_pair(void *smem_dst, const void *tmap, uint32_t bar_cl, int c0, int c1, int c2) {
-  asm volatile(
-      "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes"
-      " [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(smem_addr(smem_dst)),
-      "l"(tmap), "r"(bar_cl), "r"(c0), "r"(c1), "r"(c2)
-      : "memory");
-}
 // Arrives on the barrier at this offset in both CTAs of the pair once every MMA this thread issued before has
 // completed.
 __device__ __forceinline__ void umma_commit_both(uint64_t *bar) {
-  asm volatile(
-      "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(smem_addr(bar)),
-      "h"((uint16_t)3)
-      : "memory");
+  umma_commit_pair(smem_addr(bar));
+  umma_commit_pair(mapa_shared(smem_addr(bar), 1));
 }
 __device__ __forceinline__ float4 ld_cluster_f32x4(uint32_t addr_cl) {
   float4 v;
