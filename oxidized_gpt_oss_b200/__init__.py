@@ -8,6 +8,10 @@ the reference runner's hot-path interface (cipher-rc5/oxidized_gpt_oss):
 * ``ffn.swiglu``              — src/ffn.rs:5 (clamped gpt-oss form)
 * ``moe.MoELayer.forward``    — src/moe.rs:16
 
+and, without a counterpart there, the MXFP4 operators: ``mxfp4.quantize_mxfp4``,
+``ffn.swiglu_quantize_mxfp4``, ``mxfp4.mxfp4_matmul`` and
+``mxfp4.mxfp4_grouped_matmul``.
+
 It holds no fallback: every call goes through the CUDA library, and loading
 fails loudly when the library or a GPU is missing.
 """
