@@ -65,7 +65,7 @@ def dequantize_mxfp4(blocks: torch.Tensor, scales: torch.Tensor, rows: int, cols
         raise ValueError(f"unsupported scale dtype {scales.dtype}")
     c = context(ctx)
     if out is None:
-        out = blocks.new_empty(max(rows * cols, 0), dtype=torch.int16)
+        out = torch.empty_strided((max(rows * cols, 0),), (1,), dtype=torch.int16, device=blocks.device)
     st = c.lib.oxg_dequant_mxfp4(c.handle, blocks.data_ptr(), blocks.numel(), scales.data_ptr(),
                                  scales.numel(), fmt, rows, cols, out.data_ptr())
     if st == abi.OXG_ERR_SHAPE:
@@ -126,6 +126,11 @@ def rows_of(x: torch.Tensor, name: str) -> tuple[torch.Tensor, int, int]:
     return x, x.shape[0], x.stride(0) if x.shape[0] > 1 else x.shape[1]
 
 
+def _empty(rows: int, cols: int, dtype: torch.dtype, device: torch.device) -> torch.Tensor:
+    """A new matrix (empty_strided is torch's quickest way to one: 1.5 us, new_empty 2.0, empty 2.4)."""
+    return torch.empty_strided((rows, cols), (cols, 1), dtype=dtype, device=device)
+
+
 def scale_rule_code(rule: str) -> int:
     if rule not in _RULES:
         raise ValueError(f"unknown scale rule {rule!r}: one of {', '.join(_RULES)}")
@@ -138,9 +143,14 @@ def quantized_like(x: torch.Tensor, cols: int, rows: int, tiled: bool) -> tuple[
         raise ValueError(f"cols must be divisible by 32, got {cols}")
     if tiled and x.dim() != 2:
         raise ValueError(f"tiled scales are those of one matrix: the input must have 2 dimensions, got {x.dim()}")
+    blocks = _empty(rows, cols // 2, torch.uint8, x.device)
+    if tiled:
+        return blocks, x.new_empty(((cols + 127) // 128, rows, 4), dtype=torch.uint8)
+    scales = _empty(rows, cols // 32, torch.uint8, x.device)
+    if x.dim() == 2:
+        return blocks, scales
     lead = x.shape[:-1]
-    shape = ((cols + 127) // 128, rows, 4) if tiled else (*lead, cols // 32)
-    return x.new_empty((*lead, cols // 2), dtype=torch.uint8), x.new_empty(shape, dtype=torch.uint8)
+    return blocks.view(*lead, cols // 2), scales.view(*lead, cols // 32)
 
 
 def quantize_mxfp4(x: torch.Tensor, *, row_scale: torch.Tensor | None = None, scale_rule: str = "floor",
@@ -212,7 +222,7 @@ def _output(out: torch.Tensor | None, out_dtype: torch.dtype, m: int, n: int, a:
     if out is None:
         if out_dtype not in (torch.float32, torch.bfloat16):
             raise ValueError(f"out_dtype must be float32 or bfloat16, got {out_dtype}")
-        return a.new_empty((m, n), dtype=out_dtype), _DTYPES[out_dtype], n
+        return _empty(m, n, out_dtype, a.device), _DTYPES[out_dtype], n
     if out.shape != (m, n) or out.dtype not in (torch.float32, torch.bfloat16) or out.device != a.device or \
             (n > 1 and out.stride(1) != 1) or (m > 1 and out.stride(0) < n):
         raise ValueError(f"out must be a float32 or bfloat16 [{m}, {n}] on {a.device} with contiguous rows")
