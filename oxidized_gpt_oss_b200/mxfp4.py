@@ -242,7 +242,8 @@ def mxfp4_matmul(a_blocks: torch.Tensor, a_scales: torch.Tensor, b_blocks: torch
                  out: torch.Tensor | None = None, ctx: abi.Context | None = None) -> torch.Tensor:
     """a [m, k] times b [n, k] transposed, plus ``bias`` [n] (bfloat16), both
     operands MXFP4 (blocks [rows, k / 2], scales tiled [ceil(k / 128), rows, 4] or
-    [rows, k / 32]); f32 sums, returned as ``out_dtype`` (float32 or bfloat16)."""
+    [rows, k / 32]); f32 sums, returned as ``out_dtype`` (float32 or bfloat16) or
+    in ``out``, in its own type (contiguous rows of any pitch)."""
     index = a_blocks.get_device()
     a_blocks, a_scales = _operand(a_blocks, a_scales, "a", 2, index, ctx)
     b_blocks, b_scales = _operand(b_blocks, b_scales, "b", 2, index, ctx)
@@ -268,7 +269,8 @@ def mxfp4_grouped_matmul(a_blocks: torch.Tensor, a_scales: torch.Tensor, counts:
     on (counts: int32 CUDA tensor, zeros allowed; ``MoELayer.dispatch`` returns
     them). bias [groups, n] bfloat16. Rows past the last group keep what ``out``
     held (nothing in particular in a new one). Counts that are negative or add
-    up to more than m are reported by the context's next ``sync``."""
+    up to more than m are reported by the context's next ``sync``
+    (``device_context(a_blocks, None).sync()`` without one of your own)."""
     index = a_blocks.get_device()
     a_blocks, a_scales = _operand(a_blocks, a_scales, "a", 2, index, ctx)
     b_blocks, b_scales = _operand(b_blocks, b_scales, "b", 3, index, ctx)

@@ -296,6 +296,17 @@ def test_matmul_scales_far_from_one_and_nan(cuda_ctx):
     assert np.array_equal(np.isnan(got), nan)
 
 
+@pytest.mark.parametrize("spread", [6, 12, 30])
+@pytest.mark.parametrize("m,n,k", [(33, 130, 64), (20, 64, 2880), (300, 256, 1056)])
+def test_matmul_scales_spread_in_a_row(cuda_ctx, m, n, k, spread):
+    """Blocks of one row up to 2^120 apart: sums that f32 does not hold exactly, within the same bound."""
+    torch, mxfp4, _ = _torch()
+    rng = np.random.default_rng(k + spread)
+    (ab, asc), (bb, bsc) = _operand(rng, m, k, spread=spread), _operand(rng, n, k, spread=spread)
+    a, at, b, bt = _cuda(ab, ref.tile(asc, k), bb, ref.tile(bsc, k))
+    _check(mxfp4.mxfp4_matmul(a, at, b, bt, out_dtype=torch.float32), ref.values(ab, asc), ref.values(bb, bsc), None, "float32")
+
+
 @pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
 @pytest.mark.parametrize("pitch,offset", [(96, 0), (97, 1), (104, 3)])
 def test_matmul_writes_its_own_elements_only(cuda_ctx, dtype, pitch, offset):
