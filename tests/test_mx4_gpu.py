@@ -524,6 +524,44 @@ def test_threads_on_streams_of_their_own(cuda_ctx):
     assert not bad
 
 
+@pytest.mark.parametrize("tokens", [1, 6, 40, 200])
+def test_in_turn_with_the_moe_kernels(cuda_ctx, tokens):
+    """Products and quantisations between MoE forwards, whose kernels overlap their neighbours' ends as these do: the
+    same bits as with a wait after every call."""
+    torch, mxfp4, _ = _torch()
+    from oxidized_gpt_oss_b200 import synth
+    from oxidized_gpt_oss_b200.moe import MoELayer
+    layer = MoELayer(synth.moe_layer(seed=8, hidden=576, intermediate=320, n_experts=8, top_k=4))
+    layer.reserve(tokens)
+    w1 = mxfp4.quantize_mxfp4(torch.randn(576, 1024, device="cuda") / 32, tiled=True)
+    w2 = mxfp4.quantize_mxfp4(torch.randn(1024, 576, device="cuda") / 24, tiled=True)
+
+    def rounds(x, wait):
+        got = []
+        for _ in range(8):
+            q = mxfp4.quantize_mxfp4(x, tiled=True)
+            wait()
+            h = mxfp4.mxfp4_matmul(*q, *w1)
+            wait()
+            y = layer.forward(h)
+            wait()
+            q = mxfp4.quantize_mxfp4(y, tiled=True)
+            wait()
+            x = mxfp4.mxfp4_matmul(*q, *w2)
+            wait()
+            got += [h, y, x]
+        return got
+
+    x = torch.randn(tokens, 1024, device="cuda", dtype=torch.bfloat16)
+    want = rounds(x, torch.cuda.synchronize)
+    for _ in range(5):
+        got = rounds(x, lambda: None)
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+    cuda_ctx.sync()
+    layer.release()
+
+
 FIRST_IN_CAPTURE = """
 import torch
 from oxidized_gpt_oss_b200 import abi, mxfp4
