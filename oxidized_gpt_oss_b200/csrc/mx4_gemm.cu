@@ -184,6 +184,10 @@ __global__ void __launch_bounds__(kThreads, 1)
     mbar_init(&mma_done, 1);
     fence_mbar_init();
   }
+  if (warp == 3 && elect_one()) {
+    prefetch_tmap(&tm_x);
+    prefetch_tmap(&tm_w);
+  }
   if (warp == 1) {
     if (PAIR) {
       tmem_alloc_pair(&tmem_slot, C::TMEM_COLS);
@@ -195,11 +199,19 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
   launch_dependents();
   wait_prerequisites();  // nothing above touches memory that an earlier kernel writes
-  if (warp == 2) {  // running sums of the groups' rows and activation tiles
+  if (warp == 2 && !p.counts) {
+    if (lane == 0) {
+      const int t = (p.m + C::NMAX - 1) / C::NMAX;
+      row0_[0] = tile0_[0] = 0;
+      row0_[1] = p.m;
+      tile0_[1] = t;
+      per_[0] = round_cols<C>((p.m + t - 1) / t);
+    }
+  } else if (warp == 2) {  // running sums of the groups' rows and activation tiles
     int rows_run = 0, tiles_run = 0;
     for (int g0 = 0; g0 < p.groups; g0 += 32) {
       const int g = g0 + lane;
-      int c = g < p.groups ? (p.counts ? __ldg(p.counts + g) : p.m) : 0;
+      int c = g < p.groups ? __ldg(p.counts + g) : 0;
       bool bad = c < 0;
       c = max(c, 0);
       long long r = c;  // rows up to and including this group's
@@ -288,11 +300,6 @@ __global__ void __launch_bounds__(kThreads, 1)
 
   if (warp == 0) {
     // ------------------------------------------------------------ codes
-    if (elect_one()) {
-      prefetch_tmap(&tm_x);
-      prefetch_tmap(&tm_w);
-    }
-    __syncwarp();
     int s = 0, round = 0;
     bool ok = true;
     for (Walk w = start(); ok && w.item < total; advance(w)) {
