@@ -23,14 +23,17 @@
 // What bounds it, and measured figures (B200; device time back to back):
 //   many rows: per stage and SM the tensor cores need 449 cycles (256 x 224 x 256 in a pair), the codes and scales
 //   come in at 34 KB (528 cycles at 64 bytes a cycle), and shared memory is written and read with some 60 KB;
-//   532 cycles measured. 8192^3: 182 us, 6.0 PFLOP/s (67 % of the kind::mxf4 rate) in bursts; for seconds on end
-//   the power cap takes the clock from 1965 to about 1455 MHz. 8192 x 5120 x 2880: 53 us, 4.6 PFLOP/s (12 stages
-//   a tile, and the ends of the launch). 32768 rows over 32 groups x 5760 x 2880: 262-278 us, 4.1 PFLOP/s.
+//   540 cycles measured (83 % of the tensor cores' rate), and at that rate the power cap takes the clock from 1965
+//   MHz to about 1500 within a launch or two. 8192^3: 182 us, 6.0 PFLOP/s. 8192 x 5120 x 2880: 53 us, 4.6 PFLOP/s
+//   (12 stages a tile, and the ends of the launch: 636 cycles a stage). 32768 rows over 32 groups x 5760 x 2880:
+//   260-320 us with the card's temperature, 3.4-4.2 PFLOP/s.
 //   few rows: HBM. 64 x 201088 x 2880: 57-62 us, 5.8-6.3 TB/s; 32 rows over 27 of 32 groups x 5760 x 2880: 44 us,
 //   5.4 TB/s, of which about 4 us are the launch, the first stage's latency and the last epilogue.
 // Tried and left out: asking L2 for the next tile's codes ahead of TMA (decode 74 us instead of 44), L2 promotion
-// of 128 bytes or none (equal), tiles of 448 activation rows in both accumulators (a third less L2 traffic, but
-// nothing to compute while an epilogue of 2600 cycles runs, and coarser rounds of tiles).
+// of 128 bytes or none (equal); taking the tensor memory only after the first loads are on their way (500 cycles
+// sooner to the first stage, 5 % slower throughout); two epilogue chunks in flight (equal). Not built: tiles of 448
+// activation rows in both accumulators (a quarter less L2 traffic, but nothing to compute while an epilogue of
+// 2600 cycles runs, and coarser rounds of tiles).
 //
 // CTAs walk their tiles with the weight tile fastest: CTAs side by side share activation rows, and a group's
 // weights stay in L2. Warps: 0 TMA (codes, 128-byte swizzle), 1 MMA, 2-3 and 12-17 scales (four for the weights'
