@@ -116,6 +116,10 @@ OXG_API int oxg_swiglu(oxg_ctx *ctx, const float *gate_dev, const float *up_dev,
  *                     oxg_mxfp4_tile_scales; the quantisers write either.
  * These calls keep nothing between them and use no workspace: calls on several
  * streams, or replays of several captured graphs, do not disturb one another.
+ * A product records what it finds wrong on the device for the context that it
+ * was called with, and that context's next oxg_sync returns it. A graph that
+ * captured products may outlive the context: it then runs as before, but what
+ * it finds is reported to nobody.
  * The same call gives the same bits every time. */
 enum { OXG_DTYPE_F32 = 0, OXG_DTYPE_BF16 = 1, OXG_DTYPE_F16 = 2 };
 /* A block with largest magnitude t in [2^e, 2^(e+1)) gets the scale 2^(e-2)

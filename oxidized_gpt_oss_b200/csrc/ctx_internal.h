@@ -64,12 +64,15 @@ bool &ctx_profile_flag(oxg_ctx *ctx);
 void ctx_add_launches(oxg_ctx *ctx, long long n);
 long long ctx_launch_count(const oxg_ctx *ctx);
 
-// The error word of the context's MXFP4 products (device; allocated with the
-// context, so no call allocates). Asking for it makes every later oxg_sync
-// read it, a captured graph's replays included.
-int *ctx_op_err(oxg_ctx *ctx);
-// Reads (and clears) it after a synchronise (mx4_abi.cu); op_err null: never asked for.
-int mx4_check_error(oxg_ctx *ctx, int *op_err);
+// The error word of the context's MXFP4 products, one of the library's own on
+// every device. Asking for it makes every later oxg_sync read it, a captured
+// graph's replays included.
+int ctx_mx4_word(oxg_ctx *ctx);
+// The words (mx4_abi.cu): one that no other context has; back, cleared, with a
+// context that ends; read (and cleared) after a synchronise. Below 0: none.
+int mx4_word_take();
+void mx4_word_give(int word);
+int mx4_check_error(oxg_ctx *ctx, int word);
 
 // Full-model state (model_abi.cu), owned by the context.
 struct ModelState;

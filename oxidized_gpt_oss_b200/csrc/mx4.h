@@ -42,6 +42,9 @@ cudaError_t launch_mx4_tile_scales(const uint8_t *src, size_t groups, size_t row
                                    cudaStream_t stream);
 
 constexpr int kMx4MaxGroups = 1024;
+// Error words of the products: part of the library's module on every device, so that a context's word costs no
+// allocation and a captured launch may outlive the context that it was captured with.
+constexpr int kMx4ErrWords = 4096;
 // Error-word codes of the products.
 constexpr int kMx4ErrWait = 81;    // a pipeline wait ran out
 constexpr int kMx4ErrCounts = 85;  // a negative group count, or counts beyond the rows there are
@@ -58,8 +61,10 @@ struct Mx4GemmArgs {
   void *out = nullptr;               // [m, ldo]
   size_t ldo = 0;
   int out_bf16 = 0;                  // else f32
-  int *err = nullptr;
+  int err_word = 0;                  // below kMx4ErrWords
 };
 cudaError_t launch_mx4_gemm(const Mx4GemmArgs &a, int n_sms, cudaStream_t stream);
+// Reads an error word of the current device, and clears it where it is set. Waits for nothing but itself.
+cudaError_t mx4_take_error(int word, int *code);
 
 }  // namespace oxg

@@ -5,6 +5,7 @@
 
 #include <cstdarg>
 #include <cstdio>
+#include <mutex>
 
 #include "../../include/oxg_b200.h"
 #include "ctx_internal.h"
@@ -12,11 +13,36 @@
 
 namespace oxg {
 
-int mx4_check_error(oxg_ctx *ctx, int *op_err) {
-  if (!op_err) return OXG_OK;
+namespace {
+// Words given back, oldest first: a graph that outlives its context may still write to that context's word, so one
+// is used again only when all have been in use.
+std::mutex words_lock;
+int words_back[kMx4ErrWords], back_first = 0, back_n = 0;  // a ring
+int words_new = 0;
+}  // namespace
+
+int mx4_word_take() {
+  std::lock_guard<std::mutex> g(words_lock);
+  if (words_new < kMx4ErrWords - 1) return words_new++;
+  if (back_n == 0) return kMx4ErrWords - 1;  // the last one is shared by what comes beyond
+  const int w = words_back[back_first];
+  back_first = (back_first + 1) % kMx4ErrWords;
+  --back_n;
+  return w;
+}
+
+void mx4_word_give(int word) {
+  if (word < 0 || word >= kMx4ErrWords - 1) return;
+  int unread;
+  if (mx4_take_error(word, &unread) != cudaSuccess) return;  // not known to be clear: it stays unused
+  std::lock_guard<std::mutex> g(words_lock);
+  words_back[(back_first + back_n++) % kMx4ErrWords] = word;
+}
+
+int mx4_check_error(oxg_ctx *ctx, int word) {
+  if (word < 0) return OXG_OK;
   int h = 0;
-  cudaError_t st = cudaMemcpy(&h, op_err, sizeof(int), cudaMemcpyDeviceToHost);
-  if (st == cudaSuccess && h) st = cudaMemset(op_err, 0, sizeof(int));
+  const cudaError_t st = mx4_take_error(word, &h);
   if (st != cudaSuccess) return ctx_error(ctx, OXG_ERR_CUDA, cudaGetErrorString(st));
   if (h == kMx4ErrCounts)
     return ctx_error(ctx, OXG_ERR_SHAPE,
@@ -103,7 +129,7 @@ int product(oxg_ctx *ctx, oxg::Mx4GemmArgs &a, int out_dtype) {
   if (!aligned(a.bias, 2)) return fail(ctx, OXG_ERR_INVALID_ARG, "bias must be 2-byte aligned");
   a.out_bf16 = out_dtype == OXG_DTYPE_BF16;
   if (!aligned(a.out, a.out_bf16 ? 2 : 4)) return fail(ctx, OXG_ERR_INVALID_ARG, "out must be aligned to its elements");
-  a.err = oxg::ctx_op_err(ctx);
+  a.err_word = oxg::ctx_mx4_word(ctx);
   return run(ctx, a.counts ? "mxfp4_grouped_matmul" : "mxfp4_matmul",
              [&] { return oxg::launch_mx4_gemm(a, oxg::ctx_n_sms(ctx), oxg::ctx_stream(ctx)); });
 }

@@ -97,8 +97,9 @@ struct Params {
   int box;          // activation rows per TMA box
   int out_bf16;
   int pair_stores;  // bf16: n is even and rows start on 4-byte boundaries
-  int *err;
+  int err_word;
 };
+__device__ int g_err_words[kMx4ErrWords];
 
 // Where a tile lies: its group's weight rows from f0, activation rows [row0, row0 + rows).
 struct Tile {
@@ -171,6 +172,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   __shared__ int cols_[STAGES];  // the MMA's N for a stage's tile, from the TMA warp
   __shared__ int tile0_[kMx4MaxGroups + 1], row0_[kMx4MaxGroups + 1], per_[kMx4MaxGroups];  // per: rows of a group's tiles
 
+  int *const err = g_err_words + p.err_word;
   const int warp = __shfl_sync(0xFFFFFFFFu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
   const uint32_t rank = PAIR || SPLIT ? cluster_ctarank() : 0u;
   uint32_t n_ranks = C::CTAS;
@@ -225,7 +227,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       r += rows_run;
       bad |= r > p.m;
-      if (bad && blockIdx.x == 0) atomicCAS(p.err, 0, kMx4ErrCounts);
+      if (bad && blockIdx.x == 0) atomicCAS(err, 0, kMx4ErrCounts);
       // counts beyond the rows there are: the groups end with the rows
       const int first = (int)min(r - c, (long long)p.m), last = (int)min(r, (long long)p.m);
       int t = (last - first + C::NMAX - 1) / C::NMAX;
@@ -311,7 +313,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int x0 = t.row0 + (PAIR ? (int)rank * half : 0);
       const uint32_t tx = (uint32_t)(C::CTAS * (kWBytes + boxes * p.box * 128));
       for (int ks = k_lo; ks < k_hi; ++ks) {
-        if (round > 0 && !(ok = mbar_wait(&empty_[s], (round - 1) & 1, p.err, kMx4ErrWait))) break;
+        if (round > 0 && !(ok = mbar_wait(&empty_[s], (round - 1) & 1, err, kMx4ErrWait))) break;
         if (elect_one()) {
           uint8_t *st = stages + s * C::BYTES;
           cols_[s] = t.cols;
@@ -339,7 +341,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       // barrier whose scales never came costs one full wait, long after any copy has landed.
       for (int i = 0; i < STAGES; ++i) {
         const int last = i < s ? round : round - 1;
-        if (last >= 0 && !mbar_wait(&full_[i], last & 1, p.err, kMx4ErrWait)) break;
+        if (last >= 0 && !mbar_wait(&full_[i], last & 1, err, kMx4ErrWait)) break;
       }
     }
   } else if (warp == 1) {
@@ -350,12 +352,12 @@ __global__ void __launch_bounds__(kThreads, 1)
       const uint32_t sfw = tmem + C::SFW_COL, sfx = tmem + C::SFX_COL;
       for (int item = item0; ok && item < total; item += step, ++j) {
         const int buf = j & 1, rr = j >> 1;
-        if (rr > 0 && !(ok = mbar_wait(&acc_empty[buf], (rr - 1) & 1, p.err, kMx4ErrWait))) break;
+        if (rr > 0 && !(ok = mbar_wait(&acc_empty[buf], (rr - 1) & 1, err, kMx4ErrWait))) break;
         tc_fence_after();
         const uint32_t d = tmem + (uint32_t)(buf * C::NMAX);
         uint32_t id0 = 0, id2 = 0;
         for (int ks = k_lo; ks < k_hi; ++ks) {
-          if (!(ok = mbar_wait(&full_[s], phase, p.err, kMx4ErrWait))) break;
+          if (!(ok = mbar_wait(&full_[s], phase, err, kMx4ErrWait))) break;
           tc_fence_after();
           if (ks == k_lo) {
             const int cols = cols_[s];
@@ -406,7 +408,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         else umma_commit(&mma_done);
       }
       __syncwarp();
-      mbar_wait(&mma_done, 0, p.err, kMx4ErrWait);
+      mbar_wait(&mma_done, 0, err, kMx4ErrWait);
     }
   } else if (warp < 4 || warp >= 4 + kEpiWarps) {
     // ------------------------------------------------------------ scales
@@ -453,7 +455,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       fetch();
       int s = first, round = 0;
       for (int i = 0; i < left; ++i) {
-        if (round > 0 && !mbar_wait(&empty_[s], (round - 1) & 1, p.err, kMx4ErrWait)) break;
+        if (round > 0 && !mbar_wait(&empty_[s], (round - 1) & 1, err, kMx4ErrWait)) break;
         uint4 *sf = reinterpret_cast<uint4 *>(stages + s * C::BYTES + kWBytes + C::X_BYTES + (X ? C::SFW : 0)) + lane;
 #pragma unroll
         for (int w = 0; w < 2; ++w)
@@ -487,7 +489,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     for (Walk w = start(); w.item < total; advance(w), ++j) {
       const Tile t = tile_of(w);
       const int buf = j & 1;
-      if (!mbar_wait(&acc_full[buf], (j >> 1) & 1, p.err, kMx4ErrWait)) break;
+      if (!mbar_wait(&acc_full[buf], (j >> 1) & 1, err, kMx4ErrWait)) break;
       tc_fence_after();
       const int f = t.f0 + q * 32 + lane;
       const bool in = f < p.n;
@@ -717,6 +719,14 @@ int clusters_at_once(int ranks, int n_sms) {
 
 }  // namespace
 
+cudaError_t mx4_take_error(int word, int *code) {
+  const size_t at = sizeof(int) * (size_t)word;
+  cudaError_t st = cudaMemcpyFromSymbol(code, g_err_words, sizeof(int), at);
+  const int none = 0;
+  if (st == cudaSuccess && *code) st = cudaMemcpyToSymbol(g_err_words, &none, sizeof(int), at);
+  return st;
+}
+
 cudaError_t launch_mx4_gemm(const Mx4GemmArgs &a, int n_sms, cudaStream_t stream) {
   if (a.m == 0 || a.n == 0 || a.groups == 0) return cudaSuccess;
   Params p{};
@@ -734,7 +744,7 @@ cudaError_t launch_mx4_gemm(const Mx4GemmArgs &a, int n_sms, cudaStream_t stream
   p.words = (a.k + 127) / 128;
   p.out_bf16 = a.out_bf16;
   p.pair_stores = a.n % 2 == 0 && (a.ldo % 2 == 0 || a.m == 1) && (uintptr_t)a.out % 4 == 0;
-  p.err = a.err;
+  p.err_word = a.err_word;
   // Which kernel: estimates in ns from launches back to back on a B200 (k 512 .. 8192, n 640 .. 20480, m 1 .. 1024,
   // codes in L2). A launch costs 4100 with single CTAs and 5000 with pairs; a stage 265 in a CTA with up to 64
   // rows, 270 in a pair with up to 128 and 300 above; adding up a split 1300 + 17 a column. For instance 448 x 2880

@@ -157,8 +157,7 @@ struct oxg_ctx {
   bool prefill_pending = false;  // a prefill ran since the error word was last read
   Profiler prof;
   oxg::ModelState *model = nullptr;  // full-model state (model_abi.cu)
-  int *op_err = nullptr;         // error word of the MXFP4 products (mx4_abi.cu)
-  bool op_used = false;          // one of them has run
+  int mx4_word = -1;             // error word of the MXFP4 products, once one has run (mx4_abi.cu)
   unsigned long long epoch = 0;  // bumped when uploaded layers or the scratch move
   // Expert-parallel receive side (oxg_moe_experts): kept apart from ws so
   // that sizing it for the received rows never discards the dispatch's
@@ -874,9 +873,9 @@ int ctx_error(oxg_ctx *ctx, int status, const char *msg) { return fail(ctx, stat
 int ctx_device(const oxg_ctx *ctx) { return ctx->device; }
 cudaStream_t ctx_stream(const oxg_ctx *ctx) { return ctx->stream; }
 int ctx_n_sms(const oxg_ctx *ctx) { return ctx->n_sms; }
-int *ctx_op_err(oxg_ctx *ctx) {
-  ctx->op_used = true;
-  return ctx->op_err;
+int ctx_mx4_word(oxg_ctx *ctx) {
+  if (ctx->mx4_word < 0) ctx->mx4_word = oxg::mx4_word_take();
+  return ctx->mx4_word;
 }
 
 int ctx_moe_forward(oxg_ctx *ctx, int layer, const uint16_t *x, int T, float *y) {
@@ -981,13 +980,6 @@ int oxg_ctx_create(int device, oxg_ctx **out) {
     return cuda_fail(nullptr, st, "cudaStreamCreate");
   }
   ctx->stream = ctx->own_stream;
-  if ((st = cudaMalloc((void **)&ctx->op_err, sizeof(int))) == cudaSuccess) st = cudaMemset(ctx->op_err, 0, sizeof(int));
-  if (st != cudaSuccess) {
-    if (ctx->op_err) cudaFree(ctx->op_err);
-    cudaStreamDestroy(ctx->own_stream);
-    delete ctx;
-    return cuda_fail(nullptr, st, "cudaMalloc(error word)");
-  }
   *out = ctx;
   return OXG_OK;
 }
@@ -1001,7 +993,7 @@ int oxg_ctx_destroy(oxg_ctx *ctx) {
   if (ctx->ws.base) cudaFree(ctx->ws.base);
   if (ctx->comb_cnt) cudaFree(ctx->comb_cnt);
   if (ctx->ep.base) cudaFree(ctx->ep.base);
-  if (ctx->op_err) cudaFree(ctx->op_err);
+  oxg::mx4_word_give(ctx->mx4_word);
   if (ctx->pipe.h2d) cudaStreamSynchronize(ctx->pipe.h2d);
   if (ctx->pipe.d2h) cudaStreamSynchronize(ctx->pipe.d2h);
   for (int b = 0; b < 2; ++b) {
@@ -1038,7 +1030,7 @@ int oxg_sync(oxg_ctx *ctx) {
   OXG_CUDA(ctx, cudaStreamSynchronize(ctx->stream), "cudaStreamSynchronize");
   int rc = read_pipeline_error(ctx);
   if (rc) return rc;
-  if ((rc = oxg::mx4_check_error(ctx, ctx->op_used ? ctx->op_err : nullptr))) return rc;
+  if ((rc = oxg::mx4_check_error(ctx, ctx->mx4_word))) return rc;
   return oxg::model_check_error(ctx);
 }
 

@@ -14,8 +14,8 @@ The way back and what 4-bit operands are for (no counterpart in the reference):
 their own (experts). The products read scales in the tiled layout
 ``[ceil(k / 128), rows, 4]``, which the quantisers write with ``tiled=True`` and
 ``tile_scales`` makes of a checkpoint's ``[rows, k / 32]``; given the latter,
-they convert it first, on every call. The first call on a device creates its
-context, which allocates: make it before a stream capture.
+they convert it first, on every call. Making a context allocates no device
+memory, so a process's first call may be captured.
 """
 from __future__ import annotations
 

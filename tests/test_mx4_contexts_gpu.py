@@ -1,0 +1,93 @@
+"""What the contexts behind the MXFP4 entry points owe their callers on a GPU: captures, threads that end, errors."""
+import os
+import subprocess
+import sys
+
+import pytest
+
+pytestmark = pytest.mark.gpu
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+
+
+def _run(program):
+    r = subprocess.run([sys.executable, "-c", program], cwd=ROOT, capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "done" in r.stdout, r.stderr[-2000:]
+
+
+FIRST_CALLS_IN_A_CAPTURE = """
+import torch
+from oxidized_gpt_oss_b200 import ffn, mxfp4
+torch.cuda.set_device(0)
+blocks = torch.randint(0, 256, (8, 64), dtype=torch.uint8, device="cuda")
+scales = torch.randint(120, 130, (8, 4), dtype=torch.uint8, device="cuda")
+gate, up = torch.randn(1000, device="cuda"), torch.randn(1000, device="cuda")
+x, w = torch.randn(70, 512, device="cuda"), torch.randn(300, 512, device="cuda")
+def work():
+    q = [mxfp4.quantize_mxfp4(t, tiled=True) for t in (x, w)]
+    return [mxfp4.dequantize_mxfp4(blocks, scales, 8, 128), ffn.swiglu(gate, up), mxfp4.mxfp4_matmul(*q[0], *q[1])]
+torch.cuda.synchronize()
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):  # no context exists yet
+    out = work()
+g.replay()
+torch.cuda.synchronize()
+assert all(torch.equal(a, b) for a, b in zip(out, work()))
+mxfp4.context().sync()
+print("done")
+"""
+
+
+def test_a_process_whose_first_calls_are_captured():
+    """Making a context allocates nothing, so the capture that makes it stands."""
+    _run(FIRST_CALLS_IN_A_CAPTURE)
+
+
+def test_a_graph_that_outlives_its_context():
+    """A product captured with a context that is gone when the graph is replayed: what it finds wrong goes to nobody's
+    memory and to nobody's sync, and its rows are as they should be."""
+    import torch
+    from oxidized_gpt_oss_b200 import abi, mxfp4
+    a, w = (mxfp4.quantize_mxfp4(torch.randn(n, 96, device="cuda"), tiled=True) for n in (40, 33))
+    w = tuple(t[None] for t in w)
+    counts = torch.tensor([40], dtype=torch.int32, device="cuda")
+    out = torch.empty(40, 33, device="cuda")
+    gone, other = abi.Context(0), abi.Context(0)
+    mxfp4.mxfp4_grouped_matmul(*a, counts, *w, out=out, ctx=gone)
+    want = mxfp4.mxfp4_grouped_matmul(*a, counts, *w, out_dtype=torch.float32, ctx=other)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        mxfp4.mxfp4_grouped_matmul(*a, counts, *w, out=out, ctx=gone)
+    gone.close()
+    later = abi.Context(0)  # would be given whatever memory a context gives back
+    mxfp4.mxfp4_grouped_matmul(*a, counts, *w, ctx=later)
+    around = [torch.zeros(1 << 10, dtype=torch.int32, device="cuda") for _ in range(64)]
+    counts.fill_(41)
+    out.zero_()
+    g.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(out, want)
+    assert not any(t.any() for t in around)
+    for ctx in (other, later, mxfp4.context()):
+        ctx.sync()
+    for ctx in (other, later):
+        ctx.close()
+
+
+def test_every_context_has_errors_of_its_own():
+    import torch
+    from oxidized_gpt_oss_b200 import abi, mxfp4
+    a, w = (mxfp4.quantize_mxfp4(torch.randn(n, 96, device="cuda"), tiled=True) for n in (40, 33))
+    w = tuple(t[None] for t in w)
+    fits, beyond = (torch.tensor([n], dtype=torch.int32, device="cuda") for n in (40, 41))
+    for _ in range(3):  # a context that ends unread leaves nothing to the next
+        ctxs = [abi.Context(0) for _ in range(20)]
+        for i, ctx in enumerate(ctxs):
+            mxfp4.mxfp4_grouped_matmul(*a, beyond if i % 3 == 0 else fits, *w, ctx=ctx)
+        for i, ctx in enumerate(ctxs[:-3]):
+            if i % 3 == 0:
+                with pytest.raises(abi.OxgError, match="count"):
+                    ctx.sync()
+            ctx.sync()
+        for ctx in ctxs:
+            ctx.close()
