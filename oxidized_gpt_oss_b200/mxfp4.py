@@ -78,20 +78,26 @@ _DTYPES = {torch.float32: abi.OXG_DTYPE_F32, torch.bfloat16: abi.OXG_DTYPE_BF16,
 _RULES = {"floor": abi.OXG_MX_FLOOR, "noclip": abi.OXG_MX_NOCLIP}
 _device_ctx: dict[int, abi.Context] = {}
 _main_thread = threading.main_thread().ident
-_other_threads = threading.local()
+# Other threads' contexts, by thread and device. They stay when a thread ends (ending one would synchronise, in the
+# middle of whatever other threads do, a capture perhaps); a later thread that is given the same identity takes them over.
+_thread_ctx: dict[tuple[int, int], abi.Context] = {}
 _MOST = 0x7FFFFE00  # rows, columns and k of a product: 32-bit numbers with room for a tile
 
 
 def device_context(x: torch.Tensor, ctx: abi.Context | None) -> abi.Context:
     """The given context, or the calling thread's own on x's device (the main
-    thread's is the process's default one), bound to torch's current stream there."""
+    thread's is the process's default one), bound to torch's current stream there.
+
+    A thread's context outlives it. What a graph that was captured in the thread
+    finds wrong in a later replay is reported by that context's ``sync``: keep
+    what ``device_context(x, None)`` returns there."""
     index = x.get_device()
     if ctx is None:
-        if threading.get_ident() != _main_thread:
-            own = _other_threads.__dict__
-            ctx = own.get(index)
+        thread = threading.get_ident()
+        if thread != _main_thread:
+            ctx = _thread_ctx.get((thread, index))
             if ctx is None:
-                ctx = own[index] = abi.Context(index)
+                ctx = _thread_ctx[thread, index] = abi.Context(index)
         elif _default_ctx is not None and _default_ctx.device == index:
             ctx = _default_ctx
         else:

@@ -91,3 +91,79 @@ def test_every_context_has_errors_of_its_own():
             ctx.sync()
         for ctx in ctxs:
             ctx.close()
+
+
+THREADS_DURING_A_CAPTURE = """
+import gc
+import threading
+import torch
+from oxidized_gpt_oss_b200 import mxfp4
+torch.cuda.set_device(0)
+x = torch.randn(70, 512, device="cuda")
+want = mxfp4.quantize_mxfp4(x, tiled=True)
+streams = [torch.cuda.Stream() for _ in range(2)]
+held = []
+for st in streams:
+    with torch.cuda.stream(st):
+        held.append(torch.empty(1, device="cuda"))  # the allocator has room beside it for the stream's next tensors
+got = []
+def work(st):
+    with torch.cuda.stream(st):
+        got.append(mxfp4.quantize_mxfp4(x, tiled=True))
+torch.cuda.synchronize()
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    mine = mxfp4.quantize_mxfp4(x, tiled=True)
+    threads = [threading.Thread(target=work, args=(st,)) for st in streams]
+    for t in threads: t.start()
+    for t in threads: t.join()
+    del threads, t
+    gc.collect()
+g.replay()
+torch.cuda.synchronize()
+assert len(got) == 2
+for q in (mine, *got):
+    assert torch.equal(q[0], want[0]) and torch.equal(q[1], want[1])
+print("done")
+"""
+
+
+def test_threads_that_begin_and_end_while_another_captures():
+    """A capture in the default mode forbids every thread what may synchronise: a thread's first call and its end do not."""
+    _run(THREADS_DURING_A_CAPTURE)
+
+
+def test_a_graph_that_outlives_the_thread_that_captured_it():
+    """What it finds wrong is reported by the context that the thread had, whose word is nobody else's."""
+    import gc
+    import threading
+    import torch
+    from oxidized_gpt_oss_b200 import abi, mxfp4
+    a, w = (mxfp4.quantize_mxfp4(torch.randn(n, 96, device="cuda"), tiled=True) for n in (40, 33))
+    w = tuple(t[None] for t in w)
+    counts = torch.tensor([40], dtype=torch.int32, device="cuda")
+    torch.cuda.synchronize()
+    held = {}
+
+    def capture():
+        st = torch.cuda.Stream()
+        with torch.cuda.stream(st):
+            mxfp4.mxfp4_grouped_matmul(*a, counts, *w)
+            st.synchronize()
+            g = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(g, stream=st):
+                mxfp4.mxfp4_grouped_matmul(*a, counts, *w)
+        held["graph"], held["ctx"] = g, mxfp4.device_context(counts, None)
+
+    t = threading.Thread(target=capture)
+    t.start()
+    t.join()
+    del t
+    gc.collect()
+    counts.fill_(41)
+    held["graph"].replay()
+    torch.cuda.synchronize()
+    mxfp4.device_context(counts, None).sync()
+    with pytest.raises(abi.OxgError, match="count"):
+        held["ctx"].sync()
+    held["ctx"].sync()
