@@ -25,7 +25,9 @@ import torch
 
 from . import abi
 
-_default_ctx = None
+_default_ctx = None  # one of the next
+_device_ctx: dict[int, abi.Context] = {}  # the main thread's, by device
+_making = threading.Lock()
 # the raw stream handle where this torch has it: the Stream object costs 3 us a call
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 
@@ -38,14 +40,24 @@ def _bind(ctx: abi.Context) -> abi.Context:
 
 
 def context(ctx: abi.Context | None = None) -> abi.Context:
-    """The given context, or a per-process default one on the current device,
-    bound to torch's current stream."""
+    """The given context, or a per-process default one (the main thread's on the
+    device that was current when it was first asked for), bound to torch's
+    current stream."""
     global _default_ctx
     if ctx is None:
         if _default_ctx is None:
-            _default_ctx = abi.Context(torch.cuda.current_device())
+            _default_ctx = _main_context(torch.cuda.current_device())
         ctx = _default_ctx
     return _bind(ctx)
+
+
+def _main_context(index: int) -> abi.Context:
+    """The main thread's context on a device. Any thread may ask for the default one."""
+    with _making:
+        ctx = _device_ctx.get(index)
+        if ctx is None:
+            ctx = _device_ctx[index] = abi.Context(index)
+        return ctx
 
 
 def dequantize_mxfp4(blocks: torch.Tensor, scales: torch.Tensor, rows: int, cols: int, *,
@@ -76,7 +88,6 @@ def dequantize_mxfp4(blocks: torch.Tensor, scales: torch.Tensor, rows: int, cols
 
 _DTYPES = {torch.float32: abi.OXG_DTYPE_F32, torch.bfloat16: abi.OXG_DTYPE_BF16, torch.float16: abi.OXG_DTYPE_F16}
 _RULES = {"floor": abi.OXG_MX_FLOOR, "noclip": abi.OXG_MX_NOCLIP}
-_device_ctx: dict[int, abi.Context] = {}
 _main_thread = threading.main_thread().ident
 # Other threads' contexts, by thread and device. They stay when a thread ends (ending one would synchronise, in the
 # middle of whatever other threads do, a capture perhaps); a later thread that is given the same identity takes them over.
@@ -98,12 +109,10 @@ def device_context(x: torch.Tensor, ctx: abi.Context | None) -> abi.Context:
             ctx = _thread_ctx.get((thread, index))
             if ctx is None:
                 ctx = _thread_ctx[thread, index] = abi.Context(index)
-        elif _default_ctx is not None and _default_ctx.device == index:
-            ctx = _default_ctx
         else:
             ctx = _device_ctx.get(index)
             if ctx is None:
-                ctx = _device_ctx[index] = abi.Context(index)
+                ctx = _main_context(index)
     elif ctx.device != index:
         raise ValueError(f"the context is on cuda:{ctx.device}, the input on {x.device}")
     return _bind(ctx)

@@ -167,3 +167,23 @@ def test_a_graph_that_outlives_the_thread_that_captured_it():
     with pytest.raises(abi.OxgError, match="count"):
         held["ctx"].sync()
     held["ctx"].sync()
+
+
+ERROR_BEFORE_THE_DEFAULT_CONTEXT = """
+import torch
+from oxidized_gpt_oss_b200 import abi, mxfp4
+torch.cuda.set_device(0)
+a, w = (mxfp4.quantize_mxfp4(torch.randn(n, 96, device="cuda"), tiled=True) for n in (40, 33))
+counts = torch.tensor([41], dtype=torch.int32, device="cuda")
+mxfp4.mxfp4_grouped_matmul(*a, counts, *(t[None] for t in w))
+mxfp4.dequantize_mxfp4(a[0], torch.zeros(40, 3, dtype=torch.uint8, device="cuda"), 40, 96)
+try:
+    mxfp4.device_context(counts, None).sync()
+except abi.OxgError as e:
+    assert e.status == abi.OXG_ERR_SHAPE
+    print("done")
+"""
+
+
+def test_an_error_is_not_lost_when_the_default_context_comes_after_it():
+    _run(ERROR_BEFORE_THE_DEFAULT_CONTEXT)
