@@ -62,11 +62,17 @@ def _main_context(index: int) -> abi.Context:
 
 def dequantize_mxfp4(blocks: torch.Tensor, scales: torch.Tensor, rows: int, cols: int, *,
                      ctx: abi.Context | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
-    """blocks: uint8 CUDA tensor; scales: int16/uint16 (bf16 bits) or uint8 (E8M0).
+    """blocks: uint8 CUDA tensor; scales: int16/uint16 (bf16 bits) or uint8 (E8M0),
+    on the same device, which the work runs on.
 
     Returns an int16 tensor of rows*cols bf16 bit patterns."""
     if not (blocks.is_cuda and scales.is_cuda):
         raise ValueError("blocks and scales must be CUDA tensors")
+    index = blocks.get_device()
+    if scales.get_device() != index:
+        raise ValueError("blocks and scales must be on one device")
+    if out is not None and out.get_device() != index and (out.is_cuda or not out.is_pinned()):
+        raise ValueError(f"out must be on cuda:{index} or in pinned host memory")
     blocks = blocks.contiguous()
     scales = scales.contiguous()
     if scales.dtype == torch.uint8:
@@ -75,7 +81,7 @@ def dequantize_mxfp4(blocks: torch.Tensor, scales: torch.Tensor, rows: int, cols
         fmt = abi.OXG_SCALE_BF16
     else:
         raise ValueError(f"unsupported scale dtype {scales.dtype}")
-    c = context(ctx)
+    c = device_context(blocks, ctx)
     if out is None:
         out = torch.empty_strided((max(rows * cols, 0),), (1,), dtype=torch.int16, device=blocks.device)
     st = c.lib.oxg_dequant_mxfp4(c.handle, blocks.data_ptr(), blocks.numel(), scales.data_ptr(),

@@ -5,14 +5,27 @@ import threading
 import time
 
 import pytest
+import torch
 
-from oxidized_gpt_oss_b200 import abi, mxfp4
+from oxidized_gpt_oss_b200 import abi, ffn, mxfp4
 
 
 class Lib:
     @staticmethod
     def oxg_ctx_set_stream(handle, stream):
         handle.append(stream)
+        return abi.OXG_OK
+
+    launched = []
+
+    @classmethod
+    def oxg_dequant_mxfp4(cls, handle, *args):
+        cls.launched.append(handle)
+        return abi.OXG_OK
+
+    @classmethod
+    def oxg_swiglu(cls, handle, *args):
+        cls.launched.append(handle)
         return abi.OXG_OK
 
 
@@ -39,8 +52,33 @@ class On:
         return self.index
 
 
+class On0(torch.Tensor):
+    """Host memory that says it is on a GPU."""
+    index, is_cuda = 0, True
+
+    def get_device(self):
+        return self.index
+
+
+class On1(On0):
+    index = 1
+
+
+def tensor(of, *shape, dtype=torch.uint8):
+    return torch.zeros(*shape, dtype=dtype).as_subclass(of)
+
+
+def read_back(of=On0, scales_of=None, **kw):
+    return mxfp4.dequantize_mxfp4(tensor(of, 2, 32), tensor(scales_of or of, 2, 2), 2, 64, **kw)
+
+
+def activate(of=On0, up_of=None, **kw):
+    return ffn.swiglu(*(tensor(o, 64, dtype=torch.float32) for o in (of, up_of or of)), **kw)
+
+
 @pytest.fixture(autouse=True)
 def stand_ins(monkeypatch):
+    Lib.launched = []
     Context.made, Context.ended, Context.numbers = [], [], itertools.count()
     monkeypatch.setattr(abi, "Context", Context)
     monkeypatch.setattr(mxfp4, "_raw_stream", lambda device: (threading.get_ident(), device))
@@ -118,3 +156,37 @@ def test_the_default_context_is_made_once():
     for t in ts:
         t.join()
     assert all(c is got[0] for c in got) and mxfp4.device_context(On(0), None) is got[0]
+
+
+@pytest.mark.parametrize("call", [read_back, activate])
+def test_another_threads_call_leaves_the_main_threads_context_alone(call):
+    """The context that the main thread has just put on its stream is not moved to another thread's before it launches."""
+    main = mxfp4.device_context(On(0), None)
+    assert main is mxfp4.context()
+    streams = list(main.handle)
+    in_thread(call)
+    assert main.handle == streams
+    assert len(Lib.launched) == 1 and Lib.launched[0] is not main.handle
+    call()
+    assert Lib.launched[1] is main.handle
+
+
+@pytest.mark.parametrize("call", [read_back, activate])
+def test_calls_run_on_their_operands_device(call):
+    """On the operands' device whichever is current, and on no other: a context of another, or operands on two, are
+    refused before anything is launched."""
+    mxfp4.context()
+    call(On1)
+    assert Lib.launched == [mxfp4.device_context(On(1), None).handle]
+    del Lib.launched[:]
+    with pytest.raises(ValueError, match="the context is on cuda:0"):
+        call(On1, ctx=mxfp4.context())
+    for operands in ((On0, On1), (On1, On0)):
+        with pytest.raises(ValueError, match="one device"):
+            call(*operands)
+    assert not Lib.launched
+    with pytest.raises(ValueError, match="out"):
+        read_back(On0, out=tensor(On1, 128, dtype=torch.int16))
+    with pytest.raises(ValueError, match="out"):
+        read_back(On0, out=torch.zeros(128, dtype=torch.int16))
+    assert not Lib.launched

@@ -187,3 +187,54 @@ except abi.OxgError as e:
 
 def test_an_error_is_not_lost_when_the_default_context_comes_after_it():
     _run(ERROR_BEFORE_THE_DEFAULT_CONTEXT)
+
+
+def test_threads_that_read_back_while_the_main_thread_multiplies():
+    """Two threads quantise and dequantise on streams of their own while the main thread's products run on a third."""
+    import threading
+    import torch
+    from oxidized_gpt_oss_b200 import ffn, mxfp4
+    x, w = torch.randn(700, 2048, device="cuda"), mxfp4.quantize_mxfp4(torch.randn(900, 2048, device="cuda"), tiled=True)
+    want = mxfp4.mxfp4_matmul(*mxfp4.quantize_mxfp4(x, tiled=True), *w)
+    mine = [torch.randn(300, 4096, device="cuda") for _ in range(2)]
+    back = [mxfp4.dequantize_mxfp4(*mxfp4.quantize_mxfp4(m), 300, 4096) for m in mine]
+    act = [ffn.swiglu(m[:, ::2], m[:, 1::2]) for m in mine]
+    torch.cuda.synchronize()
+    bad, gate = [], threading.Barrier(3)
+
+    def work(m, b, y):
+        with torch.cuda.stream(torch.cuda.Stream()) as _:
+            st = torch.cuda.current_stream()
+            gate.wait()
+            for _ in range(150):
+                got, h = mxfp4.dequantize_mxfp4(*mxfp4.quantize_mxfp4(m), 300, 4096), ffn.swiglu(m[:, ::2], m[:, 1::2])
+                st.synchronize()
+                if not (torch.equal(got, b) and torch.equal(h, y)):
+                    bad.append("thread")
+
+    threads = [threading.Thread(target=work, args=a) for a in zip(mine, back, act)]
+    for t in threads:
+        t.start()
+    st = torch.cuda.Stream()
+    gate.wait()
+    with torch.cuda.stream(st):
+        for _ in range(150):
+            got = mxfp4.mxfp4_matmul(*mxfp4.quantize_mxfp4(x, tiled=True), *w)
+            st.synchronize()
+            if not torch.equal(got, want):
+                bad.append("main")
+    for t in threads:
+        t.join()
+    assert not bad
+
+
+def test_dequantize_into_pinned_memory():
+    import torch
+    from oxidized_gpt_oss_b200 import mxfp4
+    b, s = mxfp4.quantize_mxfp4(torch.randn(8, 64, device="cuda"))
+    out = torch.empty(8 * 64, dtype=torch.int16, pin_memory=True)
+    mxfp4.dequantize_mxfp4(b, s, 8, 64, out=out)
+    torch.cuda.synchronize()
+    assert torch.equal(out.cuda(), mxfp4.dequantize_mxfp4(b, s, 8, 64))
+    with pytest.raises(ValueError, match="pinned"):
+        mxfp4.dequantize_mxfp4(b, s, 8, 64, out=torch.empty(8 * 64, dtype=torch.int16))
