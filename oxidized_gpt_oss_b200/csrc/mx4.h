@@ -16,6 +16,45 @@ namespace oxg {
 // this covers every kernel before it.
 __device__ __forceinline__ void launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 __device__ __forceinline__ void wait_prerequisites() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
+// Loads of what an earlier kernel may have written, for behind that wait: this kernel may have been resident while
+// the earlier one still wrote, so the non-coherent path (ld.global.nc, __ldg), which is for data that nothing writes
+// while a kernel runs, is not for them. It costs the same (8192 x 2880 quantised from bf16: 10.9 us with
+// either, 64 x 201088 x 2880 product: 61.4).
+__device__ __forceinline__ uint4 ld_stream_v4(const void *p) {
+  uint4 r;
+  asm volatile("ld.global.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w)
+               : "l"(p));
+  return r;
+}
+__device__ __forceinline__ uint32_t ld_u32(const void *p) {
+  uint32_t r;
+  asm volatile("ld.global.u32 %0, [%1];" : "=r"(r) : "l"(p));
+  return r;
+}
+__device__ __forceinline__ uint32_t ld_u32_if(bool go, const void *p) {  // 0 where not
+  uint32_t r;
+  asm volatile(
+      "{\n\t.reg .pred q;\n\t"
+      "setp.ne.b32 q, %2, 0;\n\t"
+      "mov.b32 %0, 0;\n\t"
+      "@q ld.global.u32 %0, [%1];\n\t}"
+      : "=&r"(r)
+      : "l"(p), "r"((int)go));
+  return r;
+}
+__device__ __forceinline__ float ld_f32(const float *p) { return __uint_as_float(ld_u32(p)); }
+__device__ __forceinline__ uint16_t ld_u16(const void *p) {
+  uint16_t r;
+  asm volatile("ld.global.u16 %0, [%1];" : "=h"(r) : "l"(p));
+  return r;
+}
+__device__ __forceinline__ uint32_t ld_u8(const void *p) {
+  uint32_t r;
+  asm volatile("ld.global.u8 %0, [%1];" : "=r"(r) : "l"(p));
+  return r;
+}
 #endif
 
 // Element types and scale rules and layouts, as the public header numbers them.

@@ -216,7 +216,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     int rows_run = 0, tiles_run = 0;
     for (int g0 = 0; g0 < p.groups; g0 += 32) {
       const int g = g0 + lane;
-      int c = g < p.groups ? __ldg(p.counts + g) : 0;
+      int c = (int)ld_u32_if(g < p.groups, p.counts + g);
       bool bad = c < 0;
       c = max(c, 0);
       long long r = c;  // rows up to and including this group's
@@ -444,7 +444,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int w = 0; w < 2; ++w) {
           const int lim = 2 * ks + w < p.words ? in : 0;
 #pragma unroll
-          for (int q = 0; q < Q; ++q) v[w][q] = 32 * q < lim ? __ldg(src + 32 * q) : 0u;
+          for (int q = 0; q < Q; ++q) v[w][q] = ld_u32_if(32 * q < lim, src + 32 * q);
           src += rows;
         }
         skip(kScaleWarps);
@@ -493,7 +493,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       tc_fence_after();
       const int f = t.f0 + q * 32 + lane;
       const bool in = f < p.n;
-      const float bias = p.bias && in && !SPLIT ? bf16_to_f32(__ldg(p.bias + (size_t)t.g * p.n + f)) : 0.f;
+      const float bias = p.bias && in && !SPLIT ? bf16_to_f32(ld_u16(p.bias + (size_t)t.g * p.n + f)) : 0.f;
       const uint32_t base = tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)(buf * C::NMAX);
       const bool whole = t.f0 + kTileW <= p.n;
       for (int c0 = 32 * half; c0 < t.rows; c0 += 64) {
@@ -572,7 +572,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       float bias[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i)
-        bias[i] = p.bias && f + i < p.n ? bf16_to_f32(__ldg(p.bias + (size_t)t.g * p.n + f + i)) : 0.f;
+        bias[i] = p.bias && f + i < p.n ? bf16_to_f32(ld_u16(p.bias + (size_t)t.g * p.n + f + i)) : 0.f;
       for (int c = (int)rank + warp * (int)n_ranks; c < t.rows; c += kThreads / 32 * (int)n_ranks) {
         const uint32_t part = smem_addr(stages) + (uint32_t)(c * kTileW + 4 * lane) * 4;
         float4 v[kMaxRanks];

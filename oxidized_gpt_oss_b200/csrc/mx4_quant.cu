@@ -45,16 +45,16 @@ struct Raw {
   __device__ __forceinline__ void load(const void *p) {
     if (VEC) {
 #pragma unroll
-      for (int i = 0; i < kWords; ++i) w[i] = ldg_stream_v4(static_cast<const uint4 *>(p) + i);
+      for (int i = 0; i < kWords; ++i) w[i] = ld_stream_v4(static_cast<const uint4 *>(p) + i);
     } else if (Elem<T>::kBytes == 4) {
       uint32_t *d = reinterpret_cast<uint32_t *>(w);
 #pragma unroll
-      for (int i = 0; i < N; ++i) d[i] = __ldg(static_cast<const uint32_t *>(p) + i);
+      for (int i = 0; i < N; ++i) d[i] = ld_u32(static_cast<const uint32_t *>(p) + i);
     } else {
       uint32_t *d = reinterpret_cast<uint32_t *>(w);
       const uint16_t *s = static_cast<const uint16_t *>(p);
 #pragma unroll
-      for (int i = 0; i < N / 2; ++i) d[i] = (uint32_t)__ldg(s + 2 * i) | ((uint32_t)__ldg(s + 2 * i + 1) << 16);
+      for (int i = 0; i < N / 2; ++i) d[i] = (uint32_t)ld_u16(s + 2 * i) | ((uint32_t)ld_u16(s + 2 * i + 1) << 16);
     }
   }
   __device__ __forceinline__ void values(float (&v)[N]) const {
@@ -312,7 +312,7 @@ __global__ void __launch_bounds__(kThreads) mx4_quantize_kernel(const Mx4QuantAr
       w = swiglu_quantize8(v, a.alpha, a.limit, a.rule, &byte);
     } else {
       if (LAY != kFlat && a.row_scale) {
-        const float f = c < n_chunks ? __ldg(a.row_scale + row[u]) : 0.f;
+        const float f = c < n_chunks ? ld_f32(a.row_scale + row[u]) : 0.f;
 #pragma unroll
         for (int i = 0; i < N; ++i) v[i] = __fmul_rn(v[i], f);
       }
@@ -336,8 +336,7 @@ __global__ void __launch_bounds__(kThreads) mx4_quantize_kernel(const Mx4QuantAr
 
 // One thread per 4-byte word, consecutive rows side by side in the output.
 __global__ void __launch_bounds__(kThreads)
-    mx4_tile_scales_kernel(const uint8_t *__restrict__ src, size_t n_words, size_t rows, uint32_t kb, uint32_t words,
-                           uint32_t *__restrict__ dst) {
+    mx4_tile_scales_kernel(const uint8_t *src, size_t n_words, size_t rows, uint32_t kb, uint32_t words, uint32_t *dst) {
   launch_dependents();
   wait_prerequisites();
   for (size_t i = (size_t)blockIdx.x * kThreads + threadIdx.x; i < n_words; i += (size_t)gridDim.x * kThreads) {
@@ -347,7 +346,7 @@ __global__ void __launch_bounds__(kThreads)
     uint32_t w = 0u;
 #pragma unroll
     for (uint32_t j = 0; j < 4; ++j)
-      if (b0 + j < kb) w |= (uint32_t)__ldg(s + j) << (8 * j);
+      if (b0 + j < kb) w |= ld_u8(s + j) << (8 * j);
     dst[i] = w;
   }
 }
