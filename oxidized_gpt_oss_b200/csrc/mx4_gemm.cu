@@ -36,9 +36,9 @@
 // 2600 cycles runs, and coarser rounds of tiles).
 //
 // CTAs walk their tiles with the weight tile fastest: CTAs side by side share activation rows, and a group's
-// weights stay in L2. Warps: 0 TMA (codes, 128-byte swizzle), 1 MMA, 2-3 and 12-17 scales (four for the weights'
-// words and four for the activations', a stage each in turn; the words of a warp's next stage are on their way
-// while it waits for that stage's memory), 4-11 epilogue (two accumulators: one tile drains while the next is computed).
+// weights stay in L2. Warps: 0 TMA (codes, 128-byte swizzle), 1 MMA, 2-3 and 12-17 scales (one for
+// each stage of the ring, both operands' words; those of a warp's next turn are on their way while it waits for the
+// stage's memory), 4-11 epilogue (two accumulators: one tile drains while the next is computed).
 // Every wait is bounded; one that runs out sets the error word and the CTA winds down.
 #include <cuda.h>
 
@@ -59,8 +59,8 @@ using namespace mxf;
 constexpr int kTileW = 128;           // weight rows per CTA
 constexpr int kStageK = 256;          // elements of K per stage: 128 bytes of codes
 constexpr int kEpiWarps = 8;           // two for each quarter of the TMEM lanes, taking 32 columns in turn
-constexpr int kScaleWarps = 4;         // for each operand; a stage belongs to one of them
-constexpr int kThreads = 32 * (2 + kEpiWarps + 2 * kScaleWarps);
+constexpr int kScaleWarps = 8;         // a stage of the ring belongs to one of them
+constexpr int kThreads = 32 * (2 + kEpiWarps + kScaleWarps);
 constexpr int kMaxRanks = 8;           // CTAs that split a tile's K (the portable cluster size)
 constexpr int kWBytes = kTileW * 128;  // a stage's weight codes
 
@@ -80,7 +80,7 @@ struct Cfg {
   static constexpr uint32_t TMEM_COLS = COLS_USED <= 128 ? 128 : (COLS_USED <= 256 ? 256 : 512);
   static_assert(COLS_USED <= 512 && X_BYTES % 1024 == 0, "tensor memory, swizzle atoms");
   static_assert(!(PAIR && SPLIT), "a pair does not split K");
-  static_assert(STAGES >= kScaleWarps, "a scale warp goes around the ring at most once a step");
+  static_assert(STAGES <= kScaleWarps, "a scale warp for each stage of the ring");
   static_assert(!SPLIT || STAGES * BYTES >= NMAX * kTileW * 4, "the split's partial sums use the stages' memory");
 };
 
@@ -126,6 +126,39 @@ __device__ __forceinline__ void umma_commit_both(uint64_t *bar) {
   umma_commit_pair(smem_addr(bar));
   umma_commit_pair(mapa_shared(smem_addr(bar), 1));
 }
+// An arrival on the other CTA's barrier and a wait for one, ordered between the two CTAs (without a scope both order
+// a CTA's own threads only).
+__device__ __forceinline__ void mbar_arrive_release_cluster(uint32_t bar_cl) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar_cl) : "memory");
+}
+__device__ __forceinline__ bool mbar_wait_acquire_cluster(uint64_t *bar, uint32_t parity, int *err, int code) {
+  const long long t0 = clock64();
+  while (true) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2, %3;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(smem_addr(bar)), "r"(parity), "r"(1000000u)
+        : "memory");
+    if (ok) return true;
+    if (clock64() - t0 > kWaitBudgetCycles) {
+      atomicCAS(err, 0, code);
+      return false;
+    }
+  }
+}
+// Copies 16 bytes of this CTA's shared memory to another CTA's and counts them on a barrier there. The copy comes after
+// what the thread has written (and fenced for the async proxy) before it, and its count is a release between the CTAs:
+// the way for rank 1 to say that its scale words are in place. An arrival with a release at cluster scope says the
+// same but holds the warp for some 1400 cycles (8192 x 5120 x 2880: 61 us against 55.4, 1037 x 2880 x 4096: 12.2
+// against 10.6).
+__device__ __forceinline__ void copy_to_peer(uint32_t dst_cl, uint32_t src, uint32_t bar_cl) {
+  asm volatile("cp.async.bulk.shared::cluster.shared::cta.mbarrier::complete_tx::bytes [%0], [%1], 16, [%2];" ::"r"(dst_cl),
+               "r"(src), "r"(bar_cl)
+               : "memory");
+}
 __device__ __forceinline__ float4 ld_cluster_f32x4(uint32_t addr_cl) {
   float4 v;
   asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
@@ -168,6 +201,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint8_t *stages = smem_raw + ((1024u - (smem_addr(smem_raw) & 1023u)) & 1023u);
   __shared__ uint64_t full_[STAGES], empty_[STAGES];
   __shared__ uint64_t acc_full[2], acc_empty[2], mma_done;
+  __shared__ __align__(16) uint8_t note_[PAIR ? STAGES : 1][16];  // where rank 1 copies to
   __shared__ uint32_t tmem_slot;
   __shared__ int cols_[STAGES];  // the MMA's N for a stage's tile, from the TMA warp
   __shared__ int tile0_[kMx4MaxGroups + 1], row0_[kMx4MaxGroups + 1], per_[kMx4MaxGroups];  // per: rows of a group's tiles
@@ -179,7 +213,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (SPLIT) asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(n_ranks));
   if (threadIdx.x == 0) {
     for (int s = 0; s < STAGES; ++s) {
-      mbar_init(&full_[s], 1 + 2 * C::CTAS);  // the codes' bytes, and both operands' scales in each CTA
+      mbar_init(&full_[s], 2);  // the codes' bytes (and rank 1's note), and this CTA's scales
       mbar_init(&empty_[s], 1);
     }
     for (int b = 0; b < 2; ++b) {
@@ -301,7 +335,11 @@ __global__ void __launch_bounds__(kThreads, 1)
     t.cols = round_cols<C>(t.rows);
     return t;
   };
-  auto rank0 = [&](uint64_t *bar) { return PAIR ? mapa_shared(smem_addr(bar), 0) : smem_addr(bar); };
+  auto rank0 = [&](void *at) { return PAIR ? mapa_shared(smem_addr(at), 0) : smem_addr(at); };
+  // a pair's barriers may be completed from either CTA
+  auto wait = [&](uint64_t *bar, uint32_t parity) {
+    return PAIR ? mbar_wait_acquire_cluster(bar, parity, err, kMx4ErrWait) : mbar_wait(bar, parity, err, kMx4ErrWait);
+  };
 
   if (warp == 0) {
     // ------------------------------------------------------------ codes
@@ -311,9 +349,9 @@ __global__ void __launch_bounds__(kThreads, 1)
       const Tile t = tile_of(w);
       const int half = t.cols / C::CTAS, boxes = (half + p.box - 1) / p.box;
       const int x0 = t.row0 + (PAIR ? (int)rank * half : 0);
-      const uint32_t tx = (uint32_t)(C::CTAS * (kWBytes + boxes * p.box * 128));
+      const uint32_t tx = (uint32_t)(C::CTAS * (kWBytes + boxes * p.box * 128)) + (PAIR ? 16u : 0u);  // rank 1's note
       for (int ks = k_lo; ks < k_hi; ++ks) {
-        if (round > 0 && !(ok = mbar_wait(&empty_[s], (round - 1) & 1, err, kMx4ErrWait))) break;
+        if (round > 0 && !(ok = wait(&empty_[s], (round - 1) & 1))) break;
         if (elect_one()) {
           uint8_t *st = stages + s * C::BYTES;
           cols_[s] = t.cols;
@@ -341,7 +379,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       // barrier whose scales never came costs one full wait, long after any copy has landed.
       for (int i = 0; i < STAGES; ++i) {
         const int last = i < s ? round : round - 1;
-        if (last >= 0 && !mbar_wait(&full_[i], last & 1, err, kMx4ErrWait)) break;
+        if (last >= 0 && !wait(&full_[i], last & 1)) break;
       }
     }
   } else if (warp == 1) {
@@ -352,12 +390,12 @@ __global__ void __launch_bounds__(kThreads, 1)
       const uint32_t sfw = tmem + C::SFW_COL, sfx = tmem + C::SFX_COL;
       for (int item = item0; ok && item < total; item += step, ++j) {
         const int buf = j & 1, rr = j >> 1;
-        if (rr > 0 && !(ok = mbar_wait(&acc_empty[buf], (rr - 1) & 1, err, kMx4ErrWait))) break;
+        if (rr > 0 && !(ok = wait(&acc_empty[buf], (rr - 1) & 1))) break;
         tc_fence_after();
         const uint32_t d = tmem + (uint32_t)(buf * C::NMAX);
         uint32_t id0 = 0, id2 = 0;
         for (int ks = k_lo; ks < k_hi; ++ks) {
-          if (!(ok = mbar_wait(&full_[s], phase, err, kMx4ErrWait))) break;
+          if (!(ok = wait(&full_[s], phase))) break;
           tc_fence_after();
           if (ks == k_lo) {
             const int cols = cols_[s];
@@ -412,18 +450,13 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
   } else if (warp < 4 || warp >= 4 + kEpiWarps) {
     // ------------------------------------------------------------ scales
-    // the weights' words or the activations', every kScaleWarps-th stage
-    const int sw = warp < 4 ? warp - 2 : warp - 2 - kEpiWarps;  // 0 .. 2 kScaleWarps - 1
-    const bool x_side = sw & 1;
-    const int first = sw >> 1;
+    // a warp for each stage of the ring: both operands' words
+    const int slot = warp < 4 ? warp - 2 : warp - 2 - kEpiWarps;  // 0 .. kScaleWarps - 1
     constexpr int XQ = (C::NMAX + 31) / 32;  // 32-row pieces of the activation rows
-    auto feed = [&](auto xs_) {
-      constexpr bool X = decltype(xs_)::value;
-      constexpr int Q = X ? XQ : 4;
-      uint32_t v[2][Q];  // the words of this warp's next stage
+    if (slot < STAGES && item0 < total) {
+      uint32_t vw[2][4], vx[2][XQ];  // the words of this warp's next stage
       Walk at = start();
-      Tile t{};
-      if (at.item < total) t = tile_of(at);
+      Tile t = tile_of(at);
       int ks = k_lo;
       auto skip = [&](int stages) {
         ks += stages;
@@ -434,54 +467,49 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         if (at.item < total) t = tile_of(at);
       };
-      skip(first);
+      skip(slot);
       auto fetch = [&] {
         if (at.item >= total) return;
-        const int rows = X ? p.m : p.n, r0 = X ? t.row0 : t.f0;
-        const int in = min(rows - r0, X ? t.cols : kTileW) - lane;  // this lane's rows 32 q < in
-        const uint32_t *src = (X ? p.a_scales : p.b_scales + (size_t)t.g * p.words * p.n) + r0 + lane + (size_t)(2 * ks) * rows;
+        const int in_w = min(p.n - t.f0, kTileW) - lane, in_x = min(p.m - t.row0, t.cols) - lane;  // this lane's rows 32 q < in
+        const uint32_t *w_src = p.b_scales + (size_t)t.g * p.words * p.n + t.f0 + lane + (size_t)(2 * ks) * p.n;
+        const uint32_t *x_src = p.a_scales + t.row0 + lane + (size_t)(2 * ks) * p.m;
 #pragma unroll
         for (int w = 0; w < 2; ++w) {
-          const int lim = 2 * ks + w < p.words ? in : 0;
+          const bool held = 2 * ks + w < p.words;
+          const int lim_w = held ? in_w : 0, lim_x = held ? in_x : 0;
 #pragma unroll
-          for (int q = 0; q < Q; ++q) v[w][q] = ld_u32_if(32 * q < lim, src + 32 * q);
-          src += rows;
+          for (int q = 0; q < 4; ++q) vw[w][q] = ld_u32_if(32 * q < lim_w, w_src + 32 * q);
+#pragma unroll
+          for (int q = 0; q < XQ; ++q) vx[w][q] = ld_u32_if(32 * q < lim_x, x_src + 32 * q);
+          w_src += p.n;
+          x_src += p.m;
         }
-        skip(kScaleWarps);
+        skip(STAGES);
       };
-      // this warp's stages
-      const int mine = item0 < total ? ((total - 1 - item0) / step + 1) * (k_hi - k_lo) - first : 0;
-      const int left = (mine + kScaleWarps - 1) / kScaleWarps;
+      const int mine = ((total - 1 - item0) / step + 1) * (k_hi - k_lo) - slot;
+      const int left = (mine + STAGES - 1) / STAGES;  // this warp's stages
+      uint4 *sf = reinterpret_cast<uint4 *>(stages + slot * C::BYTES + kWBytes + C::X_BYTES) + lane;
       fetch();
-      int s = first, round = 0;
-      for (int i = 0; i < left; ++i) {
-        if (round > 0 && !mbar_wait(&empty_[s], (round - 1) & 1, err, kMx4ErrWait)) break;
-        uint4 *sf = reinterpret_cast<uint4 *>(stages + s * C::BYTES + kWBytes + C::X_BYTES + (X ? C::SFW : 0)) + lane;
+      for (int round = 0; round < left; ++round) {
+        if (round > 0 && !wait(&empty_[slot], (round - 1) & 1)) break;
 #pragma unroll
-        for (int w = 0; w < 2; ++w)
+        for (int w = 0; w < 2; ++w) {
+          sf[w * (kAtomBytes / 16)] = make_uint4(vw[w][0], vw[w][1], vw[w][2], vw[w][3]);
 #pragma unroll
-          for (int q = 0; q < Q; q += 4)
-            sf[(X ? C::X_GROUPS * w + q / 4 : w) * (kAtomBytes / 16)] =
-                make_uint4(v[w][q], q + 1 < Q ? v[w][q + 1 < Q ? q + 1 : q] : 0u, q + 2 < Q ? v[w][q + 2 < Q ? q + 2 : q] : 0u,
-                           q + 3 < Q ? v[w][q + 3 < Q ? q + 3 : q] : 0u);
-        // The tensor cores read this CTA's own shared memory, which the fence has made ready for them before
-        // the barrier (rank 0's, in a pair) can move; a release at cluster scope would wait for the loads
-        // above as well (104 against 79 us at 8192 x 5120 x 2880).
-        fence_proxy_async_smem();
+          for (int q = 0; q < XQ; q += 4)
+            sf[(C::SFW + (C::X_GROUPS * w + q / 4) * kAtomBytes) / 16] =
+                make_uint4(vx[w][q], q + 1 < XQ ? vx[w][q + 1 < XQ ? q + 1 : q] : 0u,
+                           q + 2 < XQ ? vx[w][q + 2 < XQ ? q + 2 : q] : 0u, q + 3 < XQ ? vx[w][q + 3 < XQ ? q + 3 : q] : 0u);
+        }
+        fence_proxy_async_smem();  // for the tensor cores
         __syncwarp();
         if (lane == 0) {
-          if (PAIR) mbar_arrive_cluster(rank0(&full_[s]));
-          else mbar_arrive(&full_[s]);
+          if (PAIR && rank != 0) copy_to_peer(rank0(note_[slot]), smem_addr(sf), rank0(&full_[slot]));
+          else mbar_arrive(&full_[slot]);
         }
         fetch();
-        if ((s += kScaleWarps) >= STAGES) {
-          s -= STAGES;
-          ++round;
-        }
       }
-    };
-    if (x_side) feed(std::true_type{});
-    else feed(std::false_type{});
+    }
   } else {
     // ------------------------------------------------------------ epilogue
     const int q = warp & 3, half = (warp - 4) >> 2;  // TMEM lane quarter; which 32-column chunks
@@ -489,7 +517,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     for (Walk w = start(); w.item < total; advance(w), ++j) {
       const Tile t = tile_of(w);
       const int buf = j & 1;
-      if (!mbar_wait(&acc_full[buf], (j >> 1) & 1, err, kMx4ErrWait)) break;
+      if (!wait(&acc_full[buf], (j >> 1) & 1)) break;
       tc_fence_after();
       const int f = t.f0 + q * 32 + lane;
       const bool in = f < p.n;
@@ -550,10 +578,11 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
         }
       }
+      if ((total - w.item - 1) / 2 < step) continue;  // nothing waits for this accumulator any more
       tc_fence_before();
       __syncwarp();
       if (lane == 0) {
-        if (PAIR) mbar_arrive_cluster(rank0(&acc_empty[buf]));
+        if (PAIR && rank != 0) mbar_arrive_release_cluster(rank0(&acc_empty[buf]));
         else mbar_arrive(&acc_empty[buf]);
       }
     }
