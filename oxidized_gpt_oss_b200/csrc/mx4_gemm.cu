@@ -46,6 +46,7 @@
 #include <atomic>
 #include <type_traits>
 
+#include "cluster_count.h"
 #include "common.cuh"
 #include "mx4.h"
 #include "mxf.cuh"
@@ -668,9 +669,35 @@ cudaError_t code_map(CUtensorMap *map, const void *base, int rank, int k, int ro
 }
 
 
+// Clusters of `ranks` CTAs that the current device holds side by side (its processing clusters are not multiples of
+// it), or what its SMs would hold where it does not say.
+template <class C>
+int clusters_at_once(int ranks, int dev, int n_sms) {
+  static ClusterCount known[kMaxRanks + 1];
+  return known[ranks].get(dev, n_sms / ranks, [&] {
+    auto kern = mx4_gemm_kernel<C>;
+    cudaLaunchConfig_t cfg{};
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = (unsigned)ranks;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.blockDim = dim3(kThreads);
+    cfg.gridDim = dim3((unsigned)(n_sms / ranks * ranks));
+    cfg.dynamicSmemBytes = C::SMEM;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    int n = 0;
+    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM) != cudaSuccess ||
+        cudaOccupancyMaxActiveClusters(&n, kern, &cfg) != cudaSuccess) {
+      cudaGetLastError();  // not the launch's error
+      n = 0;
+    }
+    return n;
+  });
+}
 
 template <class C>
-cudaError_t launch_cfg(const Mx4GemmArgs &a, Params &p, int n_sms, int ranks, cudaStream_t stream) {
+cudaError_t launch_cfg(const Mx4GemmArgs &a, Params &p, int n_sms, int dev, int ranks, cudaStream_t stream) {
   constexpr int kTile = kTileW * C::CTAS;
   p.n_tiles = (a.n + kTile - 1) / kTile;
   // no more activation tiles than this, whatever the counts are
@@ -686,8 +713,6 @@ cudaError_t launch_cfg(const Mx4GemmArgs &a, Params &p, int n_sms, int ranks, cu
   if (tiles > 0x3FFFFFFF || tiles * p.k_steps > 0x7FFFFFFF) return cudaErrorInvalidValue;  // no GPU's memory holds such operands
   auto kern = mx4_gemm_kernel<C>;
   static std::atomic<uint64_t> ready{0};  // a bit for each device (of the first 64) that knows the attribute
-  int dev = 0;
-  if ((st = cudaGetDevice(&dev))) return st;
   if (dev >= 64 || !(ready.load(std::memory_order_relaxed) >> dev & 1)) {
     if ((st = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM))) return st;
     if (dev < 64) ready.fetch_or(1ull << dev, std::memory_order_relaxed);
@@ -705,14 +730,7 @@ cudaError_t launch_cfg(const Mx4GemmArgs &a, Params &p, int n_sms, int ranks, cu
   cfg.attrs = attr;
   cfg.numAttrs = C::SPLIT || C::PAIR ? 2 : 1;
   long long at_once = n_sms;  // tiles in work side by side; the GPU's clusters may not hold every SM
-  if (C::PAIR) {
-    static const int pairs = [&] {
-      int n = 0;
-      cfg.gridDim = dim3((unsigned)(n_sms / 2 * 2));
-      return cudaOccupancyMaxActiveClusters(&n, kern, &cfg) == cudaSuccess && n > 0 ? n : 1;
-    }();
-    at_once = std::min(pairs, n_sms / 2);
-  }
+  if (C::PAIR) at_once = std::min(clusters_at_once<C>(2, dev, n_sms), n_sms / 2);
   cfg.gridDim = dim3((unsigned)(C::SPLIT ? tiles * ranks : C::CTAS * std::min(at_once, tiles)));
   return cudaLaunchKernelEx(&cfg, kern, tm_x, tm_w, p);
 }
@@ -720,31 +738,6 @@ cudaError_t launch_cfg(const Mx4GemmArgs &a, Params &p, int n_sms, int ranks, cu
 using Pair = Cfg<true, 224, 6, false>;
 using Few = Cfg<false, 64, 8, false>;
 using FewSplit = Cfg<false, 64, 8, true>;
-
-// Clusters of `ranks` CTAs that the GPU holds side by side (its processing clusters are not multiples of it).
-int clusters_at_once(int ranks, int n_sms) {
-  static std::atomic<int> known[kMaxRanks + 1];
-  int n = known[ranks].load(std::memory_order_relaxed);
-  if (n) return n;
-  auto kern = mx4_gemm_kernel<FewSplit>;
-  cudaLaunchConfig_t cfg{};
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = (unsigned)ranks;
-  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-  cfg.blockDim = dim3(kThreads);
-  cfg.gridDim = dim3((unsigned)(n_sms / ranks * ranks));
-  cfg.dynamicSmemBytes = FewSplit::SMEM;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, FewSplit::SMEM) != cudaSuccess ||
-      cudaOccupancyMaxActiveClusters(&n, kern, &cfg) != cudaSuccess || n < 1) {
-    cudaGetLastError();
-    n = 1;
-  }
-  known[ranks].store(n, std::memory_order_relaxed);
-  return n;
-}
 
 }  // namespace
 
@@ -758,6 +751,9 @@ cudaError_t mx4_take_error(int word, int *code) {
 
 cudaError_t launch_mx4_gemm(const Mx4GemmArgs &a, int n_sms, cudaStream_t stream) {
   if (a.m == 0 || a.n == 0 || a.groups == 0) return cudaSuccess;
+  int dev = 0;
+  const cudaError_t st = cudaGetDevice(&dev);
+  if (st) return st;
   Params p{};
   p.m = a.m;
   p.n = a.n;
@@ -789,14 +785,14 @@ cudaError_t launch_mx4_gemm(const Mx4GemmArgs &a, int n_sms, cudaStream_t stream
   int ranks = 1;
   for (int r = 2; r <= kMaxRanks && 2 * r <= p.k_steps && r * few_tiles <= n_sms; ++r) {
     const double ns = 4100 + (p.k_steps + r - 1) / r * 265. + 1300 + 17. * std::min<long long>(rows, Few::NMAX);
-    if (ns < few_ns && few_tiles <= clusters_at_once(r, n_sms)) {
+    if (ns < few_ns && few_tiles <= clusters_at_once<FewSplit>(r, dev, n_sms)) {
       few_ns = ns;
       ranks = r;
     }
   }
-  if (pair_ns < few_ns) return launch_cfg<Pair>(a, p, n_sms, 1, stream);
-  if (ranks > 1) return launch_cfg<FewSplit>(a, p, n_sms, ranks, stream);
-  return launch_cfg<Few>(a, p, n_sms, 1, stream);
+  if (pair_ns < few_ns) return launch_cfg<Pair>(a, p, n_sms, dev, 1, stream);
+  if (ranks > 1) return launch_cfg<FewSplit>(a, p, n_sms, dev, ranks, stream);
+  return launch_cfg<Few>(a, p, n_sms, dev, 1, stream);
 }
 
 }  // namespace oxg
