@@ -88,6 +88,9 @@ constexpr int kMx4ErrWords = 4096;
 constexpr int kMx4ErrWait = 81;    // a pipeline wait ran out
 constexpr int kMx4ErrCounts = 85;  // a negative group count, or counts beyond the rows there are
 
+// The products' kernels: single CTAs, pairs of them, clusters that split K.
+enum { kMx4Auto = -1, kMx4Few = 0, kMx4Pair = 1, kMx4Split = 2 };
+
 struct Mx4GemmArgs {
   int m = 0, n = 0, k = 0;           // activation rows, weight rows (per group), reduction length
   int groups = 1;
@@ -101,6 +104,8 @@ struct Mx4GemmArgs {
   size_t ldo = 0;
   int out_bf16 = 0;                  // else f32
   int err_word = 0;                  // below kMx4ErrWords
+  int kernel = kMx4Auto, ranks = 0;  // for tests: this kernel whatever the sizes; CTAs that split K
+  int *ran = nullptr;                // for tests: the kernel taken, and its ranks
 };
 cudaError_t launch_mx4_gemm(const Mx4GemmArgs &a, int n_sms, cudaStream_t stream);
 // Reads an error word of the current device, and clears it where it is set. Waits for nothing but itself.

@@ -227,4 +227,34 @@ int oxg_mxfp4_grouped_matmul(oxg_ctx *ctx, const uint8_t *a_blocks, const uint8_
   return product(ctx, a, out_dtype);
 }
 
+// Not part of the interface: either product with a kernel of the caller's choice (-1: the library's own), for tests that
+// hold every kernel to the same sizes. ran: the kernel taken and the CTAs that split its K. groups < 0: not grouped.
+__attribute__((visibility("default"))) int oxgtest_mxfp4_product(oxg_ctx *ctx, const uint8_t *a_blocks, const uint8_t *a_scales,
+                                                                 int m, const int32_t *counts_dev, int groups,
+                                                                 const uint8_t *b_blocks, const uint8_t *b_scales, int n, int k,
+                                                                 const uint16_t *bias, void *out, int out_dtype, size_t ldo,
+                                                                 int kernel, int ranks, int *ran) {
+  if (!ctx) return fail(nullptr, OXG_ERR_INVALID_ARG, "ctx is NULL");
+  if (kernel < oxg::kMx4Auto || kernel > oxg::kMx4Split) return fail(ctx, OXG_ERR_INVALID_ARG, "unknown kernel %d", kernel);
+  if (groups > oxg::kMx4MaxGroups || (groups > 0 && !counts_dev))
+    return fail(ctx, OXG_ERR_INVALID_ARG, "groups without counts, or too many");
+  oxg::Mx4GemmArgs a{};
+  a.m = m;
+  a.n = n;
+  a.k = k;
+  a.groups = groups < 0 ? 1 : groups;
+  a.counts = groups < 0 ? nullptr : counts_dev;
+  a.a = a_blocks;
+  a.a_scales = reinterpret_cast<const uint32_t *>(a_scales);
+  a.b = b_blocks;
+  a.b_scales = reinterpret_cast<const uint32_t *>(b_scales);
+  a.bias = bias;
+  a.out = out;
+  a.ldo = ldo;
+  a.kernel = kernel;
+  a.ranks = ranks;
+  a.ran = ran;
+  return product(ctx, a, out_dtype);
+}
+
 }  // extern "C"

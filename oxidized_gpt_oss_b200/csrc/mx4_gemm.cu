@@ -790,8 +790,19 @@ cudaError_t launch_mx4_gemm(const Mx4GemmArgs &a, int n_sms, cudaStream_t stream
       ranks = r;
     }
   }
-  if (pair_ns < few_ns) return launch_cfg<Pair>(a, p, n_sms, dev, 1, stream);
-  if (ranks > 1) return launch_cfg<FewSplit>(a, p, n_sms, dev, ranks, stream);
+  int kernel = pair_ns < few_ns ? kMx4Pair : (ranks > 1 ? kMx4Split : kMx4Few);
+  if (a.kernel != kMx4Auto) {
+    kernel = a.kernel;
+    ranks = a.ranks;
+    // every rank has a stage to add, or the sums would be waited for in vain
+    if (kernel == kMx4Split && (ranks < 2 || ranks > kMaxRanks || ranks > p.k_steps)) return cudaErrorInvalidValue;
+  }
+  if (a.ran) {
+    a.ran[0] = kernel;
+    a.ran[1] = kernel == kMx4Split ? ranks : 1;
+  }
+  if (kernel == kMx4Pair) return launch_cfg<Pair>(a, p, n_sms, dev, 1, stream);
+  if (kernel == kMx4Split) return launch_cfg<FewSplit>(a, p, n_sms, dev, ranks, stream);
   return launch_cfg<Few>(a, p, n_sms, dev, 1, stream);
 }
 
