@@ -42,7 +42,8 @@ def _bind(ctx: abi.Context) -> abi.Context:
 def context(ctx: abi.Context | None = None) -> abi.Context:
     """The given context, or a per-process default one (the main thread's on the
     device that was current when it was first asked for), bound to torch's
-    current stream."""
+    current stream. A context serves one thread at a time: a MoE layer that is
+    called from other threads than the main one wants a context of its own."""
     global _default_ctx
     if ctx is None:
         if _default_ctx is None:
@@ -66,10 +67,10 @@ def dequantize_mxfp4(blocks: torch.Tensor, scales: torch.Tensor, rows: int, cols
     on the same device, which the work runs on.
 
     Returns an int16 tensor of rows*cols bf16 bit patterns."""
-    if not (blocks.is_cuda and scales.is_cuda):
-        raise ValueError("blocks and scales must be CUDA tensors")
     index = blocks.get_device()
-    if scales.get_device() != index:
+    if index < 0 or scales.get_device() != index:
+        if not (blocks.is_cuda and scales.is_cuda):
+            raise ValueError("blocks and scales must be CUDA tensors")
         raise ValueError("blocks and scales must be on one device")
     if out is not None and out.get_device() != index and (out.is_cuda or not out.is_pinned()):
         raise ValueError(f"out must be on cuda:{index} or in pinned host memory")
@@ -81,7 +82,7 @@ def dequantize_mxfp4(blocks: torch.Tensor, scales: torch.Tensor, rows: int, cols
         fmt = abi.OXG_SCALE_BF16
     else:
         raise ValueError(f"unsupported scale dtype {scales.dtype}")
-    c = device_context(blocks, ctx)
+    c = _context_on(index, ctx)
     if out is None:
         out = torch.empty_strided((max(rows * cols, 0),), (1,), dtype=torch.int16, device=blocks.device)
     st = c.lib.oxg_dequant_mxfp4(c.handle, blocks.data_ptr(), blocks.numel(), scales.data_ptr(),
@@ -108,7 +109,10 @@ def device_context(x: torch.Tensor, ctx: abi.Context | None) -> abi.Context:
     A thread's context outlives it. What a graph that was captured in the thread
     finds wrong in a later replay is reported by that context's ``sync``: keep
     what ``device_context(x, None)`` returns there."""
-    index = x.get_device()
+    return _context_on(x.get_device(), ctx)
+
+
+def _context_on(index: int, ctx: abi.Context | None) -> abi.Context:
     if ctx is None:
         thread = threading.get_ident()
         if thread != _main_thread:
@@ -120,7 +124,7 @@ def device_context(x: torch.Tensor, ctx: abi.Context | None) -> abi.Context:
             if ctx is None:
                 ctx = _main_context(index)
     elif ctx.device != index:
-        raise ValueError(f"the context is on cuda:{ctx.device}, the input on {x.device}")
+        raise ValueError(f"the context is on cuda:{ctx.device}, the input on cuda:{index}")
     return _bind(ctx)
 
 
@@ -274,7 +278,7 @@ def mxfp4_matmul(a_blocks: torch.Tensor, a_scales: torch.Tensor, b_blocks: torch
         raise ValueError(f"a has rows of {k} elements, b of {2 * b_blocks.shape[1]}")
     out, code, ldo = _output(out, out_dtype, m, n, a_blocks)
     bias = _bias(bias, (n,), index)
-    c = device_context(a_blocks, ctx)
+    c = _context_on(index, ctx)
     check_status(c.lib.oxg_mxfp4_matmul(c.handle, a_blocks.data_ptr(), a_scales.data_ptr(), m, b_blocks.data_ptr(),
                                         b_scales.data_ptr(), n, k, None if bias is None else bias.data_ptr(),
                                         out.data_ptr(), code, ldo), c)
@@ -305,7 +309,7 @@ def mxfp4_grouped_matmul(a_blocks: torch.Tensor, a_scales: torch.Tensor, counts:
     counts = counts.contiguous()
     out, code, ldo = _output(out, out_dtype, m, n, a_blocks)
     bias = _bias(bias, (groups, n), index)
-    c = device_context(a_blocks, ctx)
+    c = _context_on(index, ctx)
     check_status(c.lib.oxg_mxfp4_grouped_matmul(c.handle, a_blocks.data_ptr(), a_scales.data_ptr(), m, counts.data_ptr(),
                                                 groups, b_blocks.data_ptr(), b_scales.data_ptr(), n, k,
                                                 None if bias is None else bias.data_ptr(), out.data_ptr(), code, ldo), c)
