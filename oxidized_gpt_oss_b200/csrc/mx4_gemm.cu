@@ -20,15 +20,14 @@
 // there are far fewer tiles than SMs, a cluster splits a tile's K and adds the parts through distributed shared
 // memory in rank order (so a result does not depend on timing).
 //
-// What bounds it, and measured figures (B200; device time back to back):
-//   many rows: per stage and SM the tensor cores need 449 cycles (256 x 224 x 256 in a pair), the codes and scales
-//   come in at 34 KB (528 cycles at 64 bytes a cycle), and shared memory is written and read with some 60 KB;
-//   540 cycles measured (83 % of the tensor cores' rate), and at that rate the power cap takes the clock from 1965
-//   MHz to about 1500 within a launch or two. 8192^3: 182 us, 6.0 PFLOP/s. 8192 x 5120 x 2880: 53 us, 4.6 PFLOP/s
-//   (12 stages a tile, and the ends of the launch: 636 cycles a stage). 32768 rows over 32 groups x 5760 x 2880:
-//   260-320 us with the card's temperature, 3.4-4.2 PFLOP/s.
-//   few rows: HBM. 64 x 201088 x 2880: 57-62 us, 5.8-6.3 TB/s; 32 rows over 27 of 32 groups x 5760 x 2880: 44 us,
-//   5.4 TB/s, of which about 4 us are the launch, the first stage's latency and the last epilogue.
+// What bounds it, and measured figures (B200; device time back to back; cycles of single launches):
+//   many rows: a stage of a pair (256 x 224 x 256) is 449 cycles of the tensor cores, and 34 KB come in for it on each
+//   SM, at up to 54 bytes a cycle where the port from L2 gives 64. 8192^3: 189 us, 5.8 PFLOP/s, tensor work in 77 % of
+//   the cycles, at 1.6 GHz under the power cap. 8192 x 5120 x 2880: 55 us, 4.4 PFLOP/s, 51 %: 100 k cycles for 120 stages
+//   in line, of which about 2400 a tile (12 stages) and 17000 a launch are not the stages'. 32768 rows over 32 groups x
+//   5760 x 2880: 265-320 us with the card's temperature, 3.4-4.1 PFLOP/s, 55 %.
+//   few rows: HBM. 64 x 201088 x 2880: 61-63 us, 5.7-5.9 TB/s; 32 rows over 27 of 32 groups x 5760 x 2880: 44-57 us,
+//   4.2-5.4 TB/s, of which about 4 us are the launch, the first stage's latency and the last epilogue.
 // Tried and left out: asking L2 for the next tile's codes ahead of TMA (decode 74 us instead of 44), L2 promotion
 // of 128 bytes or none (equal); taking the tensor memory only after the first loads are on their way (500 cycles
 // sooner to the first stage, 5 % slower throughout); two epilogue chunks in flight (equal). Not built: tiles of 448

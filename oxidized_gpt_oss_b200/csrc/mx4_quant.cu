@@ -181,7 +181,9 @@ __device__ __forceinline__ double swiglu_f64(float gf, float uf, float alpha, fl
 // block's largest magnitude or a scaled element lies within kTol of a border between two scales or two codes
 // (the latter seen by rounding both (1 - kTol) and (1 + kTol) times the value), or where one of these conditions
 // does not hold, the block's four lanes evaluate it again in f64: about 1 block in 300 of normally distributed
-// inputs. The codes then do not depend on which exponential computed them.
+// inputs. The codes then do not depend on which exponential computed them. Gates far out cost more: 32768 x 2880 from
+// bf16 takes 93 us (tiled scales) with gates of deviation 2, 124 with 5, 312 with 8 and 470 where every block has one
+// below -23.
 constexpr float kTol = 0x1p-17f;
 __device__ __forceinline__ uint32_t swiglu_quantize8_f64(const float (&gu)[16], float alpha, float limit, int rule, int *byte,
                                                       uint32_t lanes) {
