@@ -10,7 +10,7 @@ from __future__ import annotations
 import torch
 
 from . import abi
-from .mxfp4 import _DTYPES, check_status, device_context, quantized_like, rows_of, scale_rule_code
+from .mxfp4 import _DTYPES, _context_on, check_status, device_context, quantized_like, rows_of, scale_rule_code
 
 ALPHA = 1.702
 LIMIT = 7.0
@@ -20,14 +20,15 @@ def swiglu(gate: torch.Tensor, up: torch.Tensor, alpha: float = ALPHA, limit: fl
            ctx: abi.Context | None = None) -> torch.Tensor:
     if gate.shape != up.shape:
         raise ValueError(f"gate and up shapes differ: {tuple(gate.shape)} vs {tuple(up.shape)}")
-    if gate.dtype != torch.float32 or up.dtype != torch.float32 or not (gate.is_cuda and up.is_cuda):
+    index = gate.get_device()
+    if gate.dtype != torch.float32 or up.dtype != torch.float32 or index < 0 or up.get_device() != index:
+        if gate.dtype == up.dtype == torch.float32 and gate.is_cuda and up.is_cuda:
+            raise ValueError("gate and up must be on one device")
         raise ValueError("gate and up must be float32 CUDA tensors")
-    if gate.get_device() != up.get_device():
-        raise ValueError("gate and up must be on one device")
     g = gate.contiguous()
     u = up.contiguous()
     out = torch.empty_like(g)
-    c = device_context(g, ctx)
+    c = _context_on(index, ctx)
     abi.check(c.lib.oxg_swiglu(c.handle, g.data_ptr(), u.data_ptr(), g.numel(), float(alpha), float(limit),
                                out.data_ptr()), c.handle)
     return out
